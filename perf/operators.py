@@ -21,6 +21,9 @@ import torch
 
 own = False
 
+# NVFP4 tensor scales, as a calibration leaves them: of weights, and of activations (f32 values)
+WEIGHT_SCALE = float(torch.tensor(0.12 / (6 * 448)))
+ACTIVATION_SCALE = float(torch.tensor(64.0 / (6 * 448)))
 BLOCK = {"mxfp8": 32, "mxfp4": 32, "nvfp4": 16}
 DTYPE = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
@@ -134,8 +137,8 @@ def _quantized(fmt, x, g):
     x = torch.nn.functional.pad(x, (0, _padded(fmt, cols) - cols)).view(rows, -1, BLOCK[fmt])
     amax = x.abs().amax(2, keepdim=True)
     if fmt == "nvfp4":
-        s = (amax / (6.0 * g)).clamp(max=448.0).to(torch.float8_e4m3fn).float()
-        q = x * torch.where(s > 0, 1.0 / (s * g), torch.zeros_like(s))
+        s = (amax * (1.0 / (6.0 * g))).clamp(max=448.0).to(torch.float8_e4m3fn).float()
+        q = torch.where(s > 0, x / (s * g), 0.0)
     else:
         # the exponent of the largest value, less that of the format's largest
         e = ((amax.view(torch.int32) >> 23) - (8 if fmt == "mxfp8" else 2)).clamp(min=0)
@@ -235,7 +238,7 @@ def prepare(case, seed):
         s["values"] = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev)
     if op == "quantize":
         s["x"] = normal(rows, cols + case["pad"], 0.02).to(ty)[:, :cols]
-        s["g"] = 0.12 / (6 * 448) if fmt == "nvfp4" else 1.0
+        s["g"] = WEIGHT_SCALE if fmt == "nvfp4" else 1.0
     elif op == "rmsnorm":
         s["x"] = activations(rows, cols).to(ty)
         s["residual"] = activations(rows, cols).to(ty) if case["residual"] else None
@@ -244,11 +247,11 @@ def prepare(case, seed):
         s["eps"] = 1e-5
     else:
         m, n, k = case["m"], case["n"], case["k"]
-        gw = 0.12 / (6 * 448) if fmt == "nvfp4" else 1.0
+        gw = WEIGHT_SCALE if fmt == "nvfp4" else 1.0
         w, w_scales = _encode(fmt, normal(n, k, 0.02), gw)
         s["tables"] = _tables(dev)
         if op == "matmul":
-            ga = 64.0 / (6 * 448) if fmt == "nvfp4" else 1.0
+            ga = ACTIVATION_SCALE if fmt == "nvfp4" else 1.0
             s["a"], s["a_scales"] = _encode(fmt, activations(m, k), ga)
             s["b"], s["b_scales"], s["alpha"] = w, w_scales, ga * gw
             s["c"] = torch.empty(m, n, dtype=ty, device=dev)
