@@ -504,6 +504,57 @@ int lyth_b200_transpose_narrow(int ty, uint32_t rows, uint32_t cols, const uint1
 int lyth_b200_reduce_partials_narrow(int op, int ty, uint64_t n, const uint16_t *x, const uint16_t *y, uint32_t grid,
                                      float *partial, cudaStream_t stream);
 
+/* ---- block-scaled ("microscaled") formats: 8- and 4-bit codes with one scale per block of a row.
+ * No reference kernel: they stand beside the GEMV's INT4 / NF4 weights and the bf16 contraction.
+ *   LYTH_MX_FP8    E4M3 codes, blocks of 32, scale 2^(byte - 127) (E8M0)    } OCP Microscaling v1.0
+ *   LYTH_MX_FP4    E2M1 codes, blocks of 32, scale 2^(byte - 127) (E8M0)    }
+ *   LYTH_MX_NVFP4  E2M1 codes, blocks of 16, scale E4M3, times one f32 scale per tensor
+ * A matrix of rows x cols is held as rows x k codes, k = cols rounded up to four blocks (128, 128,
+ * 64 columns), zero behind cols. Codes: row-major, lyth_b200_mx_row_bytes(fmt, cols) bytes a row, in
+ * 4 bits the even column in a byte's low half. Scales: lyth_b200_mx_scale_bytes(fmt, rows, cols)
+ * bytes in tiles of 128 rows x 4 blocks, 512 bytes each, a tile row's tiles along k, then the next
+ * 128 rows; row r, block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b. Scale bytes of rows behind
+ * the last are neither written nor used. A code stands for code * scale (* tensor scale).
+ * Quantisation: the MX scale is the exponent of the block's largest magnitude less that of the
+ * largest code (at least 2^-127); the NVFP4 scale is that magnitude / (6 * tensor_scale) rounded to
+ * E4M3 (at most 448). Codes are value / scale rounded to nearest even and saturated. A block that
+ * holds an infinity or a NaN gets the NaN scale (0xFF, 0x7F) and zero codes.
+ * `ty` is the type of the unquantised side: LYTH_MX_F32, LYTH_NARROW_F16 or LYTH_NARROW_BF16. Row
+ * strides (ld*) count elements; rows that start on 16 bytes take vector accesses. Codes and scales
+ * start on 16 bytes (else LYTH_E_UNSUPPORTED). Zero rows are fine and do nothing; zero columns, a
+ * stride below the width, or a tensor scale outside 2^-100 .. 2^100 (MX formats: other than 1) are
+ * LYTH_E_INVALID. */
+#define LYTH_MX_FP8 0
+#define LYTH_MX_FP4 1
+#define LYTH_MX_NVFP4 2
+#define LYTH_MX_F32 0
+uint64_t lyth_b200_mx_row_bytes(int fmt, uint32_t cols);
+uint64_t lyth_b200_mx_scale_bytes(int fmt, uint64_t rows, uint32_t cols);
+/* codes, scales = x (rows x cols of `ty`). */
+int lyth_b200_quantize_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const void *x, uint64_t ldx,
+                          float tensor_scale, uint8_t *codes, uint8_t *scales, cudaStream_t stream);
+/* out (rows x cols of `ty`) = the values that codes and scales stand for, rounded once to the type. */
+int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const uint8_t *codes, const uint8_t *scales,
+                            float tensor_scale, void *out, uint64_t ldo, cudaStream_t stream);
+/* h = x + residual; codes, scales = h / sqrt(mean(h^2) + eps) * weight, quantised; residual_out = h
+ * rounded to the type. All in f32 between the loads and the two roundings. residual and
+ * residual_out may be null (h = x; h not written), and residual_out may be x or residual. */
+int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const void *x, uint64_t ldx,
+                         const void *residual, uint64_t ldr, void *residual_out, uint64_t ldo, const void *weight,
+                         float eps, float tensor_scale, uint8_t *codes, uint8_t *scales, cudaStream_t stream);
+/* c (m x n of `ty`) = alpha * a b^T: a is m x cols, b n x cols, both in `fmt`; f32 accumulation on
+ * the block-scaled tensor cores (tcgen05.mma .block_scale), rounded once. alpha carries the tensor
+ * scales. Any m, n, cols; m or n zero does nothing. */
+int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, const uint8_t *a,
+                        const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, float alpha, void *c,
+                        uint64_t ldc, cudaStream_t stream);
+/* y (m x n) = alpha * x w^T for a few rows of unquantised x: x is m x cols of `ty` (f16 or bf16),
+ * m <= LYTH_GEMV_MX_MAX_M, w n x cols in `fmt`; f32 accumulation, y rounded once to `ty`. */
+#define LYTH_GEMV_MX_MAX_M 8
+int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, const void *x, uint64_t ldx,
+                      const uint8_t *w, const uint8_t *w_scales, float alpha, void *y, uint64_t ldy,
+                      cudaStream_t stream);
+
 /* ---- the back-end entry: a lowered kernel in, a kernel of this library (or a refusal) out.
  * Replaces lyth_ptx::emit(&KernelIr, arch) -> Module (crates/lyth-ptx/src/lib.rs:65-253; refusals
  * EmitError, :48-62) and Function::launch_shared with Arg slots in declaration order

@@ -135,6 +135,14 @@ _sig("lyth_b200_device_error", _i32, [])
 _sig("lyth_b200_stream_narrow", _i32, [_i32, _i32, _u64, C.POINTER(_f32), _vp, _vp, _vp, _vp])
 _sig("lyth_b200_transpose_narrow", _i32, [_i32, _u32, _u32, _vp, _vp, _vp])
 _sig("lyth_b200_reduce_partials_narrow", _i32, [_i32, _i32, _u64, _vp, _vp, _u32, _vp, _vp])
+_sig("lyth_b200_mx_row_bytes", _u64, [_i32, _u32])
+_sig("lyth_b200_mx_scale_bytes", _u64, [_i32, _u64, _u32])
+_sig("lyth_b200_quantize_mx", _i32, [_i32, _i32, _u64, _u32, _vp, _u64, _f32, _vp, _vp, _vp])
+_sig("lyth_b200_dequantize_mx", _i32, [_i32, _i32, _u64, _u32, _vp, _vp, _f32, _vp, _u64, _vp])
+_sig("lyth_b200_rmsnorm_mx", _i32, [_i32, _i32, _u64, _u32, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _f32, _f32, _vp, _vp,
+                                    _vp])
+_sig("lyth_b200_matmul_mx", _i32, [_i32, _i32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _f32, _vp, _u64, _vp])
+_sig("lyth_b200_gemv_mx", _i32, [_i32, _i32, _u32, _u32, _u32, _vp, _u64, _vp, _vp, _f32, _vp, _u64, _vp])
 _sig("lyth_b200_wait_selftest", _i32, [_i32, _u32, _vp])
 _sig("lyth_b200_fused_layout_selftest", _i32, [_u64, _u32, C.POINTER(_u32), C.POINTER(_u32)])
 
@@ -370,6 +378,163 @@ def gemv_dequant(fmt: int, w, scales, out, group: int = 64, stream=None) -> None
     check(lib.lyth_b200_gemv_dequant(fmt, rows, 2 * half_k, group, _ptr(w, torch.uint8, "w"),
                                      _ptr(scales, torch.float16, "scales"), _ptr(out, _f32t(), "out"),
                                      _stream(stream)), "gemv_dequant")
+
+
+# ----------------------------------------------------------------------------- block-scaled formats
+MX_FP8, MX_FP4, MX_NVFP4 = 0, 1, 2
+GEMV_MX_MAX_M = 8
+
+
+def mx_row_bytes(fmt: int, cols: int) -> int:
+    """Bytes of one row of codes: cols rounded up to four blocks, 8 or 4 bits each."""
+    return int(lib.lyth_b200_mx_row_bytes(fmt, cols))
+
+
+def mx_scale_bytes(fmt: int, rows: int, cols: int) -> int:
+    """Bytes of the tiled scales of a rows x cols matrix."""
+    return int(lib.lyth_b200_mx_scale_bytes(fmt, rows, cols))
+
+
+def mx_empty(fmt: int, rows: int, cols: int, device):
+    """Codes (rows x row bytes) and scales (flat) for a rows x cols matrix, uninitialised."""
+    import torch
+
+    return (torch.empty(rows, mx_row_bytes(fmt, cols), dtype=torch.uint8, device=device),
+            torch.empty(mx_scale_bytes(fmt, rows, cols), dtype=torch.uint8, device=device))
+
+
+_MX_TY = None
+
+
+def _mx_ty(t, name):
+    """The C ABI's code of an unquantised tensor's type."""
+    global _MX_TY
+    if _MX_TY is None:
+        import torch
+
+        _MX_TY = {torch.float32: 0, torch.float16: NARROW_F16, torch.bfloat16: NARROW_BF16}
+    ty = _MX_TY.get(t.dtype)
+    if ty is None:
+        raise TypeError(f"{name}: float32, float16 or bfloat16, got {t.dtype}")
+    return ty
+
+
+def _mx_rows(t, name, dev=None, dtype=None):
+    """(pointer, row stride) of a 2-D CUDA tensor whose rows are contiguous; any row stride."""
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must live on a CUDA device (lyth_b200 has no CPU path)")
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name}: on cuda:{t.get_device()}, the current device is cuda:{dev}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected two dimensions, got {t.dim()}")
+    rows, cols = t.shape
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    if rows < 2:
+        ld = cols
+    elif ld < cols:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, width {cols})")
+    return t.data_ptr(), ld
+
+
+def _mx_operand(fmt, rows, cols, codes, scales, dev, name):
+    """Pointers of a quantised rows x cols matrix, its sizes checked against the format's."""
+    import torch
+
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"{name}: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
+    if codes.get_device() != dev or scales.get_device() != dev:
+        raise ValueError(f"{name}: codes and scales must live on the current device, cuda:{dev}")
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError(f"{name}: codes and scales must be contiguous")
+    nb, ns = lib.lyth_b200_mx_row_bytes(fmt, cols), lib.lyth_b200_mx_scale_bytes(fmt, rows, cols)
+    if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] != nb:
+        raise ValueError(f"{name}: {rows} x {cols} takes codes of {rows} x {nb} bytes, got {tuple(codes.shape)}")
+    if scales.numel() != ns:
+        raise ValueError(f"{name}: {rows} x {cols} takes {ns} bytes of scales, got {scales.numel()}")
+    return codes.data_ptr(), scales.data_ptr()
+
+
+def _mx_device() -> int:
+    import torch
+
+    return torch.cuda.current_device()
+
+
+def quantize_mx(fmt: int, x, codes, scales, tensor_scale: float = 1.0, stream=None) -> None:
+    """codes, scales = x in a block-scaled format; x 2-D float32 / float16 / bfloat16 with contiguous
+    rows (any row stride), codes and scales as mx_empty gives them. tensor_scale: NVFP4 only."""
+    dev = _mx_device()
+    rows, cols = x.shape
+    xp, ldx = _mx_rows(x, "x", dev)
+    cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
+    check(lib.lyth_b200_quantize_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, tensor_scale, cp, sp, _stream(stream)),
+          "quantize_mx")
+
+
+def dequantize_mx(fmt: int, codes, scales, out, tensor_scale: float = 1.0, stream=None) -> None:
+    """out = the values codes and scales stand for, rounded once to out's type."""
+    dev = _mx_device()
+    rows, cols = out.shape
+    op, ldo = _mx_rows(out, "out", dev)
+    cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
+    check(lib.lyth_b200_dequantize_mx(fmt, _mx_ty(out, "out"), rows, cols, cp, sp, tensor_scale, op, ldo,
+                                      _stream(stream)), "dequantize_mx")
+
+
+def rmsnorm_mx(fmt: int, x, weight, codes, scales, residual=None, residual_out=None, eps: float = 1e-6,
+               tensor_scale: float = 1.0, stream=None) -> None:
+    """h = x + residual (f32); codes, scales = h / sqrt(mean(h^2) + eps) * weight quantised;
+    residual_out = h rounded to x's type (it may be x or residual itself)."""
+    dev = _mx_device()
+    rows, cols = x.shape
+    xp, ldx = _mx_rows(x, "x", dev)
+    rp = op = None
+    ldr = ldo = 0
+    for t, name in ((residual, "residual"), (residual_out, "residual_out")):
+        if t is not None and tuple(t.shape) != (rows, cols):
+            raise ValueError(f"{name}: expected {rows} x {cols}, got {tuple(t.shape)}")
+    if residual is not None:
+        rp, ldr = _mx_rows(residual, "residual", dev, x.dtype)
+    if residual_out is not None:
+        op, ldo = _mx_rows(residual_out, "residual_out", dev, x.dtype)
+    if weight.dim() != 1 or weight.shape[0] != cols or weight.get_device() != dev:
+        raise ValueError(f"weight: expected {cols} values on cuda:{dev}, got {tuple(weight.shape)} on {weight.device}")
+    cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
+    check(lib.lyth_b200_rmsnorm_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, rp, ldr, op, ldo,
+                                   _ptr(weight, x.dtype, "weight"), eps, tensor_scale, cp, sp, _stream(stream)),
+          "rmsnorm_mx")
+
+
+def matmul_mx(fmt: int, a, a_scales, b, b_scales, c, alpha: float = 1.0, stream=None) -> None:
+    """c = alpha * a @ b.T on the block-scaled tensor cores: a (m rows) and b (n rows) are codes in one
+    format and of one width, c m x n float32 / float16 / bfloat16 with contiguous rows."""
+    dev = _mx_device()
+    m, n = c.shape
+    cols = a.shape[-1] * (1 if fmt == MX_FP8 else 2)
+    cp, ldc = _mx_rows(c, "c", dev)
+    ap, asp = _mx_operand(fmt, m, cols, a, a_scales, dev, "a")
+    bp, bsp = _mx_operand(fmt, n, cols, b, b_scales, dev, "b")
+    check(lib.lyth_b200_matmul_mx(fmt, _mx_ty(c, "c"), m, n, cols, ap, asp, bp, bsp, alpha, cp, ldc, _stream(stream)),
+          "matmul_mx")
+
+
+def gemv_mx(fmt: int, x, w, w_scales, y, alpha: float = 1.0, stream=None) -> None:
+    """y = alpha * x @ w.T for up to GEMV_MX_MAX_M rows of float16 / bfloat16 x (m x cols); w holds
+    n x cols in a block-scaled format, y is m x n of x's type."""
+    dev = _mx_device()
+    m, cols = x.shape
+    m2, n = y.shape
+    if m2 != m:
+        raise ValueError(f"gemv shapes {tuple(x.shape)} -> {tuple(y.shape)}")
+    xp, ldx = _mx_rows(x, "x", dev)
+    yp, ldy = _mx_rows(y, "y", dev, x.dtype)
+    wp, wsp = _mx_operand(fmt, n, cols, w, w_scales, dev, "w")
+    check(lib.lyth_b200_gemv_mx(fmt, _mx_ty(x, "x"), m, n, cols, xp, ldx, wp, wsp, alpha, yp, ldy, _stream(stream)),
+          "gemv_mx")
 
 
 # ----------------------------------------------------------------------------- gates

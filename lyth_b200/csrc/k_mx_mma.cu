@@ -1,0 +1,324 @@
+// Product of two block-scaled matrices on the sm_100a tensor cores: C = alpha * A * B^T with A
+// (m x k) and B (n x k) in one of mx.cuh's formats, f32 accumulation in tensor memory, C in f32,
+// f16 or bf16. tcgen05.mma .block_scale multiplies the codes and applies both operands' block scales
+// inside the contraction, so nothing is dequantised.
+//
+// One persistent CTA per SM, 192 threads, warp-specialised as the bf16 contraction (k_mma.cu):
+//   warp 0     producer: per step of 128 bytes along k (128 E4M3 or 256 E2M1 codes), a 128-row box of
+//              A and of B (128-byte swizzle) and both operands' scale tiles (512 bytes per 128 rows x
+//              4 blocks, already in the order tensor memory wants) into a ring.
+//   warp 1     one thread copies the step's scale tiles to tensor memory (tcgen05.cp 32x128b, spread to
+//              the four lane quadrants) and issues one MMA per 32 bytes of k; tcgen05.cp and
+//              tcgen05.mma of one thread run in order, so the scales need no wait of their own.
+//   warps 2-5  epilogue: tcgen05.ld, times alpha, rounded once, stored; two accumulators let it run
+//              beside the next tile's main loop.
+// Ragged edges: rows behind m or n arrive as zeros (tensor-map fill) or carry any scale, and are not
+// stored; k is whole scale words, so the last step's MMAs are only fewer. Every wait is bounded.
+#include <cuda.h>
+
+#include "mbar.cuh"
+#include "mx.cuh"
+
+namespace lyth {
+
+__device__ int g_mx_error = 0;
+
+constexpr int XM_BM = 128, XM_BN = 128, XM_STAGES = 6, XM_THREADS = 192;
+constexpr int XM_OP_BYTES = 128 * 128;         // one operand's box: 128 rows x 128 bytes
+constexpr int XM_TMEM_COLS = 512;              // two 128-column accumulators, then the scales
+constexpr uint32_t XM_SF_COL = 2 * XM_BN;
+
+// Scale tiles (4 blocks along k) in one 128-byte step.
+template <int FMT>
+struct Xm {
+    static constexpr int kTiles = FMT == LYTH_MX_FP8 ? 1 : FMT == LYTH_MX_FP4 ? 2 : 4;
+    static constexpr int kStageBytes = 2 * XM_OP_BYTES + 2 * kTiles * 512;
+    static constexpr size_t kSmem = 1024 + (size_t)XM_STAGES * kStageBytes + 256;
+};
+
+// Instruction descriptor of the block-scaled kinds: B scale id at bits 4-5, A type at 7-9, B type at
+// 10-12 (E4M3 0 of mxf8f6f4, E2M1 1 of the 4-bit kinds), both operands K-major, N >> 3 at 17-22,
+// scale type at 23 (E8M0 1, E4M3 0), M >> 7 at 27-28, A scale id at 29-30. The scale id says which
+// bytes of the 32-bit scale cells an MMA uses: one (E4M3 codes), two, or all four (NVFP4).
+template <int FMT>
+LYTH_D uint32_t xm_idesc(int n, int m, int j) {
+    const uint32_t ty = FMT == LYTH_MX_FP8 ? 0u : 1u;
+    const uint32_t id = FMT == LYTH_MX_FP8 ? (uint32_t)j : FMT == LYTH_MX_FP4 ? (uint32_t)(j & 1) * 2u : 0u;
+    return (id << 4) | (ty << 7) | (ty << 10) | ((uint32_t)(n >> 3) << 17) |
+           ((FMT == LYTH_MX_NVFP4 ? 0u : 1u) << 23) | ((uint32_t)(m >> 7) << 27) | (id << 29);
+}
+
+LYTH_D bool xm_wait(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, &g_mx_error); }
+
+// Shared-memory descriptors: K-major rows of 128 bytes with the 128-byte swizzle (8-row groups 1024
+// bytes apart), and the unswizzled 32 x 16-byte scale tile (8-row groups 128 bytes apart).
+LYTH_D uint64_t xm_desc_op(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+}
+LYTH_D uint64_t xm_desc_sf(uint32_t addr) { return (uint64_t)((addr >> 4) & 0x3FFFu) | 8ull << 32 | 1ull << 46; }
+
+LYTH_D void xm_copy_sf(uint32_t tmem, uint32_t smem) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(xm_desc_sf(smem)) : "memory");
+}
+
+template <int FMT>
+LYTH_D void xm_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+#define LYTH_XM_MMA(KIND)                                                                                  \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                         \
+                 "tcgen05.mma.cta_group::1." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),       \
+                 "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)                                \
+                 : "memory")
+    if constexpr (FMT == LYTH_MX_FP8) LYTH_XM_MMA("kind::mxf8f6f4.block_scale.scale_vec::1X");
+    else if constexpr (FMT == LYTH_MX_FP4) LYTH_XM_MMA("kind::mxf4.block_scale.scale_vec::2X");
+    else LYTH_XM_MMA("kind::mxf4nvf4.block_scale.scale_vec::4X");
+#undef LYTH_XM_MMA
+}
+LYTH_D void xm_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+LYTH_D void xm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+LYTH_D void xm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+LYTH_D void xm_tma(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+LYTH_D void xm_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+struct XmArgs {
+    const uint8_t *sa, *sb;  // scale tiles
+    uint64_t m, n, ldc;
+    uint32_t row_bytes;      // bytes of a row of codes
+    uint32_t words;          // scale tiles along k
+    float alpha;
+    bool vec;                // rows of C start on 16 bytes
+};
+
+// 32 accumulators of one row to C, columns col .. col + 31.
+template <int TY>
+LYTH_D void xm_store32(typename MxElem<TY>::type *crow, uint64_t col, uint64_t n, bool vec, float alpha,
+                       const uint32_t (&r)[32]) {
+    if (col >= n) return;
+    const uint32_t left = n - col < 32 ? (uint32_t)(n - col) : 32u;
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = __fmul_rn(alpha, __uint_as_float(r[8 * v + i]));
+        mx_store8<TY>(crow + col, 8 * v, left, vec, f);
+    }
+}
+
+template <int FMT, int TY>
+__global__ void __launch_bounds__(XM_THREADS, 1)
+    mx_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                  typename MxElem<TY>::type *C, XmArgs p) {
+    constexpr int T = Xm<FMT>::kTiles;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = sA + XM_STAGES * XM_OP_BYTES, *sSA = sB + XM_STAGES * XM_OP_BYTES;
+    uint8_t *sSB = sSA + XM_STAGES * T * 512;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + XM_STAGES * T * 512);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * XM_STAGES + 4);
+    auto full = [&](int s) { return smem_u32(bars + s); };
+    auto empty = [&](int s) { return smem_u32(bars + XM_STAGES + s); };
+    auto tfull = [&](int b) { return smem_u32(bars + 2 * XM_STAGES + b); };
+    auto tempty = [&](int b) { return smem_u32(bars + 2 * XM_STAGES + 2 + b); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t tiles_m = (p.m + XM_BM - 1) / XM_BM, tiles_n = (p.n + XM_BN - 1) / XM_BN, ntiles = tiles_m * tiles_n;
+    const uint32_t steps = (p.row_bytes + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < XM_STAGES; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(tfull(b), 1);
+            mbar_init(tempty(b), 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(XM_TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    xm_fence_before();
+    __syncthreads();
+    xm_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (uint64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
+                const uint64_t tm = tile % tiles_m, tn = tile / tiles_m;
+                const uint8_t *sa = p.sa + tm * p.words * 512, *sb = p.sb + tn * p.words * 512;
+                for (uint32_t kb = 0; kb < steps; kb++) {
+                    if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
+                    const uint32_t w0 = kb * T, nw = p.words - w0 < T ? p.words - w0 : T;
+                    mbar_expect_tx(full(stage), 2 * XM_OP_BYTES + 2 * nw * 512);
+                    xm_tma(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), (int)(tm * XM_BM), full(stage));
+                    xm_tma(smem_u32(sB + stage * XM_OP_BYTES), &tmB, (int)(kb * 128), (int)(tn * XM_BN), full(stage));
+                    bulk_load(smem_u32(sSA + stage * T * 512), sa + (uint64_t)w0 * 512, nw * 512, full(stage));
+                    bulk_load(smem_u32(sSB + stage * T * 512), sb + (uint64_t)w0 * 512, nw * 512, full(stage));
+                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+            // After a timed-out wait, give the stages this thread may have in flight a bounded
+            // chance to land before the block leaves.
+            if (!ok) {
+                for (int s = 0; s < XM_STAGES; s++) {
+                    xm_wait(full(stage), phase);
+                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0, local = 0;
+            bool ok = true;
+            for (uint64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, local++) {
+                const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
+                if (!xm_wait(tempty(ab), aphase ^ 1)) break;
+                xm_fence_after();
+                const uint32_t d = tmem_base + ab * XM_BN;
+                for (uint32_t kb = 0; kb < steps; kb++) {
+                    if (!xm_wait(full(stage), phase)) { ok = false; break; }
+                    xm_fence_after();
+                    const uint32_t left = p.row_bytes - kb * 128;
+                    const int mmas = left < 128 ? (int)(left / 32) : 4;
+                    const uint32_t sfa = tmem_base + XM_SF_COL + (kb & 1) * 32, sfb = sfa + 16;
+                    const uint32_t a = smem_u32(sA + stage * XM_OP_BYTES), b = smem_u32(sB + stage * XM_OP_BYTES);
+#pragma unroll
+                    for (int t = 0; t < T; t++) {
+                        if (t * (4 / T) < mmas) {
+                            xm_copy_sf(sfa + 4 * t, smem_u32(sSA + (stage * T + t) * 512));
+                            xm_copy_sf(sfb + 4 * t, smem_u32(sSB + (stage * T + t) * 512));
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (j < mmas)
+                            xm_mma<FMT>(d, xm_desc_op(a + 32 * j), xm_desc_op(b + 32 * j), xm_idesc<FMT>(XM_BN, XM_BM, j),
+                                        sfa + 4 * (j * T / 4), sfb + 4 * (j * T / 4), (kb | (uint32_t)j) != 0);
+                    }
+                    xm_commit(empty(stage));
+                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (ok) xm_commit(tfull(ab));
+            }
+        }
+    } else {
+        const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may read
+        uint32_t local = 0;
+        for (uint64_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, local++) {
+            const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
+            if (!xm_wait(tfull(ab), aphase)) break;
+            xm_fence_after();
+            const uint64_t row = tile % tiles_m * XM_BM + quad * 32 + lane, n0 = tile / tiles_m * XM_BN;
+#pragma unroll 1
+            for (int c = 0; c < XM_BN / 32; c++) {
+                uint32_t r[32];
+                xm_ld32(tmem_base + ab * XM_BN + ((quad * 32) << 16) + c * 32, r);
+                if (row < p.m) xm_store32<TY>(C + row * p.ldc, n0 + c * 32, p.n, p.vec, p.alpha, r);
+            }
+            xm_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty(ab));
+        }
+    }
+    xm_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        xm_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(XM_TMEM_COLS)
+                     : "memory");
+    }
+}
+
+// Codes as a 2-D byte tensor: a 128-byte (the swizzle span) x box_rows box, zeros outside.
+static bool xm_map(CUtensorMap *map, const void *base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows) {
+    PFN_encode_tiled enc = tensor_map_encoder();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {row_bytes, rows};
+    cuuint64_t strides[1] = {row_bytes};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int TY>
+static int xm_launch(const CUtensorMap &ta, const CUtensorMap &tb, void *c, const XmArgs &p, cudaStream_t s) {
+    static bool done[64] = {false};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return status_of(e);
+    if (dev < 0 || dev >= 64 || !done[dev]) {
+        e = cudaFuncSetAttribute(mx_mma_kernel<FMT, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Xm<FMT>::kSmem);
+        if (e != cudaSuccess) return status_of(e);
+        if (dev >= 0 && dev < 64) done[dev] = true;
+    }
+    const uint64_t tiles = (p.m + XM_BM - 1) / XM_BM * ((p.n + XM_BN - 1) / XM_BN);
+    const uint64_t sms = (uint64_t)device_sms();
+    const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
+    mx_mma_kernel<FMT, TY><<<grid, XM_THREADS, Xm<FMT>::kSmem, s>>>(ta, tb, static_cast<typename MxElem<TY>::type *>(c), p);
+    return last_launch_status();
+}
+
+int mx_take_device_error() {
+    int v = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_mx_error, sizeof(int));
+    if (e != cudaSuccess) return status_of(e);
+    if (!v) return LYTH_OK;
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_mx_error, &zero, sizeof(int));
+    return LYTH_E_TIMEOUT;
+}
+
+}  // namespace lyth
+
+using namespace lyth;
+
+extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, const uint8_t *a,
+                                   const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, float alpha,
+                                   void *c, uint64_t ldc, cudaStream_t s) {
+    if (!mx_known(fmt) || !mx_ty_known(ty)) return LYTH_E_UNSUPPORTED;
+    if (cols == 0 || cols > (1u << 30) || m > (1u << 31) || n > (1u << 31) || ldc < n) return LYTH_E_INVALID;
+    if (m == 0 || n == 0) return LYTH_OK;
+    if (!a || !a_scales || !b || !b_scales || !c) return LYTH_E_INVALID;
+    if (!aligned16(a) || !aligned16(a_scales) || !aligned16(b) || !aligned16(b_scales)) return LYTH_E_UNSUPPORTED;
+    const uint64_t k = mx_padded(fmt, cols);
+    XmArgs p;
+    p.sa = a_scales;
+    p.sb = b_scales;
+    p.m = m;
+    p.n = n;
+    p.ldc = ldc;
+    p.row_bytes = (uint32_t)mx_code_bytes(fmt, k);
+    p.words = (uint32_t)(k / (4 * mx_block(fmt)));
+    p.alpha = alpha;
+    p.vec = aligned16(c) && ldc * mx_ty_bytes(ty) % 16 == 0;
+    CUtensorMap ta, tb;
+    if (!xm_map(&ta, a, p.row_bytes, m, XM_BM) || !xm_map(&tb, b, p.row_bytes, n, XM_BN)) return LYTH_E_UNSUPPORTED;
+    LYTH_MX_DISPATCH(fmt, ty, return (xm_launch<FMT, TY>(ta, tb, c, p, s)));
+    return LYTH_E_UNSUPPORTED;
+}

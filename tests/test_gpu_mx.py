@@ -1,0 +1,233 @@
+"""The block-scaled formats on the device against tests/mxref.py (64 bits, from the definition):
+quantisation and the way back bit for bit, the norm, the tensor-core product and the few-row product
+within tolerances that count their roundings."""
+import numpy as np
+import pytest
+import torch
+
+import lyth_b200 as lb
+from tests import mxref as mx
+
+pytestmark = pytest.mark.gpu
+
+FMTS = [lb.MX_FP8, lb.MX_FP4, lb.MX_NVFP4]
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+SENTINEL = 0xA5
+
+
+def empty(fmt, rows, cols, cuda):
+    codes, scales = lb.mx_empty(fmt, rows, cols, cuda)
+    codes.fill_(SENTINEL)
+    scales.fill_(SENTINEL)
+    return codes, scales
+
+
+def wide(t):
+    return t.double().cpu().numpy()
+
+
+def check_quantized(fmt, codes, scales, want_codes, want_scales):
+    rows, blocks = want_scales.shape
+    assert np.array_equal(codes.cpu().numpy(), mx.pack(fmt, want_codes))
+    # rows behind the last keep what they held
+    assert np.array_equal(scales.cpu().numpy(), mx.tile(want_scales, SENTINEL))
+
+
+def sample(rows, cols, ty, seed, cuda):
+    """Normal values over many magnitudes, with exact halfway values among them."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((rows, cols)) * np.exp2(rng.integers(-9, 9, (rows, 1)))
+    half = rng.integers(-60, 61, (rows, cols)) / 8.0
+    x = np.where(rng.random((rows, cols)) < 0.3, half, x)
+    return torch.from_numpy(x.astype(np.float32)).to(cuda).to(ty)
+
+
+# one value; less than a block; a scale word; odd widths; more rows than a scale tile; long rows
+SHAPES = [(1, 1), (1, 31), (3, 64), (5, 129), (33, 96), (129, 200), (130, 1024), (257, 4101), (2, 20000), (700, 33)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantize_bit_exact(cuda, fmt, ty, rows, cols):
+    x = sample(rows, cols, ty, 5 + rows + cols, cuda)
+    if fmt == lb.MX_NVFP4 and ty == torch.float32:
+        x = x.bfloat16().float()  # f32 of more bits can lie within f32 rounding of a code's border
+    codes, scales = empty(fmt, rows, cols, cuda)
+    lb.quantize_mx(fmt, x, codes, scales)
+    check_quantized(fmt, codes, scales, *mx.quantize(fmt, wide(x)))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("off,pad", [(0, 3), (1, 0), (8, 8), (5, 11)])
+def test_quantize_strided_rows(cuda, fmt, off, pad):
+    rows, cols = 70, 333
+    x = sample(rows, off + cols + pad, torch.bfloat16, 9, cuda)[:, off:off + cols]
+    codes, scales = empty(fmt, rows, cols, cuda)
+    lb.quantize_mx(fmt, x, codes, scales)
+    check_quantized(fmt, codes, scales, *mx.quantize(fmt, wide(x)))
+    out = torch.full((rows, off + cols + pad), 7.0, dtype=torch.float32, device=cuda)
+    lb.dequantize_mx(fmt, codes, scales, out[:, off:off + cols])
+    want = mx.values(fmt, *mx.quantize(fmt, wide(x)))[:, :cols]
+    assert np.array_equal(wide(out)[:, off:off + cols], want)
+    assert (out[:, :off] == 7).all() and (out[:, off + cols:] == 7).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_extreme_values(cuda, fmt):
+    # zeros of both signs, the smallest and largest f32, subnormals, halfway codes, infinities, NaN:
+    # one kind in each block, so a bad block's neighbours keep their values
+    b = mx.BLOCK[fmt]
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((12, 8 * b)).astype(np.float32)
+    big = np.finfo(np.float32).max
+    specials = [0.0, -0.0, 1e-45, -1e-45, 1.1754944e-38, big, -big, np.inf, -np.inf, np.nan, 2.0 ** -120, 3e38, 448.0, 0.75]
+    for i in range(x.shape[0]):
+        for j in range(0, 8, 2):
+            x[i, j * b:(j + 1) * b] = x[i, j * b:(j + 1) * b] * np.float32(0.0 if (i + j) % 3 else 1e-40)
+            x[i, j * b + int(rng.integers(b))] = specials[(4 * i + j // 2) % len(specials)]
+    if fmt == lb.MX_NVFP4:
+        x = torch.from_numpy(x).bfloat16().float().numpy()
+    xd = torch.from_numpy(x).to(cuda)
+    codes, scales = empty(fmt, *x.shape, cuda)
+    lb.quantize_mx(fmt, xd, codes, scales)
+    check_quantized(fmt, codes, scales, *mx.quantize(fmt, x.astype(np.float64)))
+
+
+@pytest.mark.parametrize("g", [0.25, 2.0 ** -14, 2.0 ** 20])
+def test_nvfp4_tensor_scale(cuda, g):
+    # powers of two: value / (6 g) and code * scale * g are exact where the definition's are
+    x = sample(40, 500, torch.bfloat16, 21, cuda)
+    codes, scales = empty(lb.MX_NVFP4, 40, 500, cuda)
+    lb.quantize_mx(lb.MX_NVFP4, x, codes, scales, tensor_scale=g)
+    wc, ws = mx.quantize(lb.MX_NVFP4, wide(x), g)
+    check_quantized(lb.MX_NVFP4, codes, scales, wc, ws)
+    out = torch.empty(40, 500, device=cuda)
+    lb.dequantize_mx(lb.MX_NVFP4, codes, scales, out, tensor_scale=g)
+    assert np.array_equal(wide(out), mx.values(lb.MX_NVFP4, wc, ws, g)[:, :500])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES)
+def test_dequantize_every_code(cuda, fmt, ty):
+    # every byte of codes under every scale byte's value that the type can tell apart
+    rows, k = 256, 4 * mx.BLOCK[fmt] * 2
+    rng = np.random.default_rng(8)
+    codes = rng.integers(0, 256 if fmt == lb.MX_FP8 else 16, (rows, k))
+    scales = np.broadcast_to(np.arange(rows)[:, None], (rows, k // mx.BLOCK[fmt])).copy()
+    if fmt == lb.MX_NVFP4:
+        scales &= 127
+    cd = torch.from_numpy(mx.pack(fmt, codes)).to(cuda)
+    sd = torch.from_numpy(mx.tile(scales)).to(cuda)
+    out = torch.empty(rows, k, dtype=ty, device=cuda)
+    lb.dequantize_mx(fmt, cd, sd, out)
+    want = mx.values(fmt, codes, scales)
+    with np.errstate(over="ignore"):
+        want = torch.from_numpy(want.astype(np.float32)).to(ty)  # f32 holds every finite product or its rounding
+    got = out.cpu()
+    same = (got == want) | (got.isnan() & want.isnan())
+    assert bool(same.all())
+
+
+def norm_ref(x, r, w, eps):
+    h = x if r is None else x + r
+    return h, h / np.sqrt((h * h).mean(1, keepdims=True) + eps) * w
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("rows,cols,residual", [(1, 4096, True), (3, 1, True), (5, 100, False), (130, 777, True), (9, 8200, True),
+                                                (4, 33000, True), (2, 70001, False)])
+def test_rmsnorm(cuda, fmt, ty, rows, cols, residual):
+    gen = torch.Generator().manual_seed(rows * 31 + cols)
+    x = torch.randn(rows, cols, generator=gen).to(ty).to(cuda)
+    r = (3 * torch.randn(rows, cols, generator=gen)).to(ty).to(cuda) if residual else None
+    w = (1 + 0.2 * torch.randn(cols, generator=gen)).to(ty).to(cuda)
+    codes, scales = empty(fmt, rows, cols, cuda)
+    h = torch.full_like(x, 9.0)
+    lb.rmsnorm_mx(fmt, x, w, codes, scales, residual=r, residual_out=h, eps=1e-5)
+    rh, ry = norm_ref(wide(x), wide(r) if residual else None, wide(w), 1e-5)
+    # h: one f32 addition, one rounding to the type
+    assert np.abs(wide(h) - rh).max() <= (np.abs(rh) * (HALF_STEP[ty] * 1.001 + 2.0 ** -24)).max()
+    # y before its rounding to codes is off by a few f32 roundings (the sum's tree has < 64 levels, then
+    # a division, an addition, rsqrtf to 2 ulp, two products): 2^-17 covers them. Quantised that is
+    # the definition's result, or a value whose code lies on the other side of a border: half a step
+    # of the code (e4m3 2^-4, e2m1 at most 1 of the scale) away from y, or one more step where the
+    # block's scale itself moved by one.
+    got = mx.values(fmt, mx.unpack(fmt, codes.cpu().numpy()), scales.cpu().numpy()[mx.scale_at(rows, mx.padded(fmt, cols) // mx.BLOCK[fmt])])[:, :cols]
+    wc, ws = mx.quantize(fmt, ry)
+    want = mx.values(fmt, wc, ws)[:, :cols]
+    lo, hi = (mx.values(fmt, *mx.quantize(fmt, ry * (1 + s * 2.0 ** -17)))[:, :cols] for s in (-1, 1))
+    bound = np.maximum(np.maximum(lo, hi), want), np.minimum(np.minimum(lo, hi), want)
+    off = (got > bound[0]) | (got < bound[1])
+    # f32 inputs have no grid: a block whose scale moved at both ends is still inside the bounds
+    assert not off.any(), (np.argwhere(off)[:4], got[off][:4], want[off][:4])
+    assert (got != want).mean() <= 1e-2
+
+
+def test_rmsnorm_in_place_and_poisoned_row(cuda):
+    rows, cols, fmt = 6, 500, lb.MX_FP8
+    for out_is in ("x", "residual"):
+        x = sample(rows, cols, torch.bfloat16, 1, cuda)
+        r = sample(rows, cols, torch.bfloat16, 2, cuda)
+        w = torch.ones(cols, dtype=torch.bfloat16, device=cuda)
+        x[3, 7] = float("nan")
+        a, b = empty(fmt, rows, cols, cuda), empty(fmt, rows, cols, cuda)
+        h = torch.empty_like(x)
+        lb.rmsnorm_mx(fmt, x, w, *a, residual=r, residual_out=h)
+        lb.rmsnorm_mx(fmt, x, w, *b, residual=r, residual_out=x if out_is == "x" else r)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.equal((x if out_is == "x" else r).view(torch.int16), h.view(torch.int16))
+        v = torch.empty(rows, cols, device=cuda)
+        lb.dequantize_mx(fmt, *a, v)
+        assert bool(v[3].isnan().all()) and bool(v[[0, 1, 2, 4, 5]].isfinite().all())
+
+
+def product_bound(a, b, alpha, k, ty):
+    """f32 accumulation of k exact products in any order, alpha's and the output's rounding. The
+    tensor cores align a step's products and may cut instead of round (up to 2^-23 of the largest
+    partial sum each step): 2 k 2^-24 of the sum of magnitudes covers a chain of k of either."""
+    s = np.abs(a) @ np.abs(b).T * abs(alpha)
+    r = np.abs(a @ b.T) * abs(alpha)
+    return s * (2 * k + 4) * 2.0 ** -24 + r * (HALF_STEP[ty] + 2.0 ** -23) + (2.0 ** -25 if ty == torch.float16 else 0)
+
+
+MM = [(1, 1, 1), (128, 128, 128), (5, 130, 64), (128, 128, 1024), (200, 136, 192), (257, 300, 1000), (1, 1000, 2048), (300, 515, 4160),
+      (33, 16, 12288), (1024, 2056, 96)]
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m,n,k", MM)
+def test_matmul(cuda, fmt, ty, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    a, sa, va = mx.random_operand(fmt, m, k, rng, 2)
+    b, sb, vb = mx.random_operand(fmt, n, k, rng, 2)
+    dev = [torch.from_numpy(t).to(cuda) for t in (a, sa, b, sb)]
+    alpha = 0.75
+    full = torch.full((m, n + 5), 3.0, dtype=ty, device=cuda)
+    c = full[:, :n]
+    lb.matmul_mx(fmt, *dev, c, alpha=alpha)
+    torch.cuda.synchronize()
+    assert lb.lib.lyth_b200_device_error() == 0
+    want = alpha * (va @ vb.T)
+    off = np.abs(wide(c) - want)
+    assert (off <= product_bound(va, vb, alpha, k, ty)).all(), (off.max(), np.argwhere(off > product_bound(va, vb, alpha, k, ty))[:4])
+    assert bool((full[:, n:] == 3).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES[1:])
+@pytest.mark.parametrize("m,n,cols", [(1, 1, 1), (1, 14336, 256), (2, 100, 64), (3, 257, 1000), (4, 128, 4101), (5, 33, 192), (8, 300, 8192),
+                                      (7, 1000, 777), (1, 64, 20000), (8, 16, 16384)])
+def test_gemv(cuda, fmt, ty, m, n, cols):
+    rng = np.random.default_rng(m + n + cols)
+    w, sw, vw = mx.random_operand(fmt, n, cols, rng, 3)
+    x = torch.from_numpy(rng.standard_normal((m, cols)).astype(np.float32)).to(ty)
+    vx = x.double().numpy()
+    y = torch.full((m, n + 3), 5.0, dtype=ty, device=cuda)
+    lb.gemv_mx(fmt, x.to(cuda), torch.from_numpy(w).to(cuda), torch.from_numpy(sw).to(cuda), y[:, :n], alpha=0.5)
+    want = 0.5 * (vx @ vw[:, :cols].T)
+    assert (np.abs(wide(y)[:, :n] - want) <= product_bound(vx, vw[:, :cols], 0.5, cols, ty)).all()
+    assert bool((y[:, n:] == 5).all())
