@@ -403,32 +403,55 @@ def mx_empty(fmt: int, rows: int, cols: int, device):
             torch.empty(mx_scale_bytes(fmt, rows, cols), dtype=torch.uint8, device=device))
 
 
-_MX_TY = None
+# The wrappers below run once per token and layer; what they look up of torch on every call is bound
+# at the first one, and a format's sizes are computed here rather than through two more C calls.
+_MX_WORD = {MX_FP8: 128, MX_FP4: 128, MX_NVFP4: 64}  # columns of a scale word: four blocks
+_MX_TY = {}
+_mx_u8 = _mx_current_device = _mx_current_stream = None
+
+
+def _mx_device() -> int:
+    """The current device; binds torch's types and queries when first asked."""
+    global _mx_u8, _mx_current_device, _mx_current_stream
+    if _mx_current_device is None:
+        import torch
+
+        _MX_TY.update({torch.float32: 0, torch.float16: NARROW_F16, torch.bfloat16: NARROW_BF16})
+        _mx_u8 = torch.uint8
+        _mx_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+        _mx_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        torch.cuda.init()
+    return _mx_current_device()
+
+
+def _mx_stream(stream, dev):
+    if stream is None:
+        return _mx_current_stream(dev)
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _mx_ty(t, name):
     """The C ABI's code of an unquantised tensor's type."""
-    global _MX_TY
-    if _MX_TY is None:
-        import torch
-
-        _MX_TY = {torch.float32: 0, torch.float16: NARROW_F16, torch.bfloat16: NARROW_BF16}
     ty = _MX_TY.get(t.dtype)
     if ty is None:
         raise TypeError(f"{name}: float32, float16 or bfloat16, got {t.dtype}")
     return ty
 
 
-def _mx_rows(t, name, dev=None, dtype=None):
+def _mx_on(t, name, dev):
+    at = t.get_device()
+    if at != dev:
+        if at < 0:
+            raise ValueError(f"{name}: must live on a CUDA device (lyth_b200 has no CPU path)")
+        raise ValueError(f"{name}: on cuda:{at}, the current device is cuda:{dev}")
+
+
+def _mx_rows(t, name, dev, dtype=None):
     """(pointer, row stride) of a 2-D CUDA tensor whose rows are contiguous; any row stride."""
-    if not t.is_cuda:
-        raise ValueError(f"{name}: must live on a CUDA device (lyth_b200 has no CPU path)")
-    if dev is not None and t.get_device() != dev:
-        raise ValueError(f"{name}: on cuda:{t.get_device()}, the current device is cuda:{dev}")
-    if dtype is not None and t.dtype != dtype:
+    _mx_on(t, name, dev)
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.dim() != 2:
-        raise ValueError(f"{name}: expected two dimensions, got {t.dim()}")
     rows, cols = t.shape
     ld, inner = t.stride()
     if inner != 1 and cols > 1:
@@ -442,47 +465,49 @@ def _mx_rows(t, name, dev=None, dtype=None):
 
 def _mx_operand(fmt, rows, cols, codes, scales, dev, name):
     """Pointers of a quantised rows x cols matrix, its sizes checked against the format's."""
-    import torch
-
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    _mx_on(codes, name, dev)
+    _mx_on(scales, name + "'s scales", dev)
+    if codes.dtype is not _mx_u8 or scales.dtype is not _mx_u8:
         raise TypeError(f"{name}: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
-    if codes.get_device() != dev or scales.get_device() != dev:
-        raise ValueError(f"{name}: codes and scales must live on the current device, cuda:{dev}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"{name}: codes and scales must be contiguous")
-    nb, ns = lib.lyth_b200_mx_row_bytes(fmt, cols), lib.lyth_b200_mx_scale_bytes(fmt, rows, cols)
-    if codes.dim() != 2 or codes.shape[0] != rows or codes.shape[1] != nb:
+    word = _MX_WORD.get(fmt)
+    if word is None:
+        raise LythError(E_UNSUPPORTED, f"{name}: format {fmt}")
+    words = -(-cols // word)
+    nb, ns = words * word >> (fmt != MX_FP8), (rows + 127 >> 7) * words << 9
+    if codes.shape != (rows, nb):
         raise ValueError(f"{name}: {rows} x {cols} takes codes of {rows} x {nb} bytes, got {tuple(codes.shape)}")
     if scales.numel() != ns:
         raise ValueError(f"{name}: {rows} x {cols} takes {ns} bytes of scales, got {scales.numel()}")
     return codes.data_ptr(), scales.data_ptr()
 
 
-def _mx_device() -> int:
-    import torch
-
-    return torch.cuda.current_device()
+def _mx_shape(t, name):
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected two dimensions, got {t.dim()}")
+    return t.shape
 
 
 def quantize_mx(fmt: int, x, codes, scales, tensor_scale: float = 1.0, stream=None) -> None:
     """codes, scales = x in a block-scaled format; x 2-D float32 / float16 / bfloat16 with contiguous
     rows (any row stride), codes and scales as mx_empty gives them. tensor_scale: NVFP4 only."""
     dev = _mx_device()
-    rows, cols = x.shape
+    rows, cols = _mx_shape(x, "x")
     xp, ldx = _mx_rows(x, "x", dev)
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
-    check(lib.lyth_b200_quantize_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, tensor_scale, cp, sp, _stream(stream)),
+    check(lib.lyth_b200_quantize_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, tensor_scale, cp, sp, _mx_stream(stream, dev)),
           "quantize_mx")
 
 
 def dequantize_mx(fmt: int, codes, scales, out, tensor_scale: float = 1.0, stream=None) -> None:
     """out = the values codes and scales stand for, rounded once to out's type."""
     dev = _mx_device()
-    rows, cols = out.shape
+    rows, cols = _mx_shape(out, "out")
     op, ldo = _mx_rows(out, "out", dev)
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
     check(lib.lyth_b200_dequantize_mx(fmt, _mx_ty(out, "out"), rows, cols, cp, sp, tensor_scale, op, ldo,
-                                      _stream(stream)), "dequantize_mx")
+                                      _mx_stream(stream, dev)), "dequantize_mx")
 
 
 def rmsnorm_mx(fmt: int, x, weight, codes, scales, residual=None, residual_out=None, eps: float = 1e-6,
@@ -490,22 +515,25 @@ def rmsnorm_mx(fmt: int, x, weight, codes, scales, residual=None, residual_out=N
     """h = x + residual (f32); codes, scales = h / sqrt(mean(h^2) + eps) * weight quantised;
     residual_out = h rounded to x's type (it may be x or residual itself)."""
     dev = _mx_device()
-    rows, cols = x.shape
+    rows, cols = _mx_shape(x, "x")
     xp, ldx = _mx_rows(x, "x", dev)
     rp = op = None
     ldr = ldo = 0
     for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None and tuple(t.shape) != (rows, cols):
+        if t is not None and t.shape != (rows, cols):
             raise ValueError(f"{name}: expected {rows} x {cols}, got {tuple(t.shape)}")
     if residual is not None:
         rp, ldr = _mx_rows(residual, "residual", dev, x.dtype)
     if residual_out is not None:
         op, ldo = _mx_rows(residual_out, "residual_out", dev, x.dtype)
-    if weight.dim() != 1 or weight.shape[0] != cols or weight.get_device() != dev:
-        raise ValueError(f"weight: expected {cols} values on cuda:{dev}, got {tuple(weight.shape)} on {weight.device}")
+    _mx_on(weight, "weight", dev)
+    if weight.shape != (cols,) or not weight.is_contiguous():
+        raise ValueError(f"weight: expected {cols} values, contiguous, got {tuple(weight.shape)}")
+    if weight.dtype is not x.dtype:
+        raise TypeError(f"weight: expected {x.dtype}, got {weight.dtype}")
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
     check(lib.lyth_b200_rmsnorm_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, rp, ldr, op, ldo,
-                                   _ptr(weight, x.dtype, "weight"), eps, tensor_scale, cp, sp, _stream(stream)),
+                                   weight.data_ptr(), eps, tensor_scale, cp, sp, _mx_stream(stream, dev)),
           "rmsnorm_mx")
 
 
@@ -513,12 +541,12 @@ def matmul_mx(fmt: int, a, a_scales, b, b_scales, c, alpha: float = 1.0, stream=
     """c = alpha * a @ b.T on the block-scaled tensor cores: a (m rows) and b (n rows) are codes in one
     format and of one width, c m x n float32 / float16 / bfloat16 with contiguous rows."""
     dev = _mx_device()
-    m, n = c.shape
-    cols = a.shape[-1] * (1 if fmt == MX_FP8 else 2)
+    m, n = _mx_shape(c, "c")
+    cols = _mx_shape(a, "a")[1] << (fmt != MX_FP8)
     cp, ldc = _mx_rows(c, "c", dev)
     ap, asp = _mx_operand(fmt, m, cols, a, a_scales, dev, "a")
     bp, bsp = _mx_operand(fmt, n, cols, b, b_scales, dev, "b")
-    check(lib.lyth_b200_matmul_mx(fmt, _mx_ty(c, "c"), m, n, cols, ap, asp, bp, bsp, alpha, cp, ldc, _stream(stream)),
+    check(lib.lyth_b200_matmul_mx(fmt, _mx_ty(c, "c"), m, n, cols, ap, asp, bp, bsp, alpha, cp, ldc, _mx_stream(stream, dev)),
           "matmul_mx")
 
 
@@ -526,14 +554,14 @@ def gemv_mx(fmt: int, x, w, w_scales, y, alpha: float = 1.0, stream=None) -> Non
     """y = alpha * x @ w.T for up to GEMV_MX_MAX_M rows of float16 / bfloat16 x (m x cols); w holds
     n x cols in a block-scaled format, y is m x n of x's type."""
     dev = _mx_device()
-    m, cols = x.shape
-    m2, n = y.shape
+    m, cols = _mx_shape(x, "x")
+    m2, n = _mx_shape(y, "y")
     if m2 != m:
         raise ValueError(f"gemv shapes {tuple(x.shape)} -> {tuple(y.shape)}")
     xp, ldx = _mx_rows(x, "x", dev)
     yp, ldy = _mx_rows(y, "y", dev, x.dtype)
     wp, wsp = _mx_operand(fmt, n, cols, w, w_scales, dev, "w")
-    check(lib.lyth_b200_gemv_mx(fmt, _mx_ty(x, "x"), m, n, cols, xp, ldx, wp, wsp, alpha, yp, ldy, _stream(stream)),
+    check(lib.lyth_b200_gemv_mx(fmt, _mx_ty(x, "x"), m, n, cols, xp, ldx, wp, wsp, alpha, yp, ldy, _mx_stream(stream, dev)),
           "gemv_mx")
 
 

@@ -159,7 +159,11 @@ class Fake:
 @pytest.fixture
 def on_device0(monkeypatch):
     monkeypatch.setattr(lb, "_mx_device", lambda: 0)
-    monkeypatch.setattr(lb, "_stream", lambda s: None)
+    monkeypatch.setattr(lb, "_mx_current_stream", lambda dev: None)
+    import torch
+
+    monkeypatch.setattr(lb, "_mx_u8", torch.uint8)
+    monkeypatch.setattr(lb, "_MX_TY", {torch.float32: 0, torch.float16: lb.NARROW_F16, torch.bfloat16: lb.NARROW_BF16})
 
 
 def held(fmt, rows, cols, dev=0):
