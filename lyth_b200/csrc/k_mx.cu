@@ -2,89 +2,133 @@
 // residual and quantises its output in the same pass.
 //
 // All three are bound by HBM: a value is read once, its code (4 or 8 bits) and a 16th to a 32nd of a
-// scale byte are written. A thread holds eight consecutive values (one 128-bit load of a 16-bit
-// type, two of f32); a block's scale needs the largest magnitude over 2 or 4 neighbouring lanes
-// (mx_quantize8), so no value is read twice and shared memory is used only for the norm's row sum.
+// scale byte are written. A thread holds sixteen consecutive values: an NVFP4 block, or half an MX
+// block whose other half is the neighbouring lane's (mx_quantize), so no value is read twice and
+// shared memory is used only for the norm's row sum.
 #include "mx.cuh"
 
 namespace lyth {
 
 constexpr int kMxThreads = 256;
 
-// Chunks (8 columns) are walked as one flat range, rows back to back: a warp's 32 chunks may lie in
-// several short rows, and a scale word's chunks never straddle a row because a row holds whole words.
-// The (row, chunk) of a thread advances by a constant step, so the only division is the first.
+// Chunks (16 columns) are one flat range, rows back to back, kMxThreads * U of them to a block: a
+// warp's 32 chunks may lie in several short rows, and a scale word's chunks never straddle a row
+// because a row holds whole words. One division finds a thread's first chunk (32-bit where the range
+// allows); the next ones are a constant step on.
 struct MxWalk {
     uint64_t row;
     uint32_t c;
-    LYTH_D MxWalk(uint64_t flat, uint32_t cpr) : row(flat / cpr), c((uint32_t)(flat % cpr)) {}
-    LYTH_D void step(uint64_t rows, uint32_t chunks, uint32_t cpr) {
+    LYTH_D MxWalk(uint64_t flat, uint32_t cpr, bool narrow) {
+        if (narrow) {
+            row = (uint32_t)flat / cpr;
+            c = (uint32_t)flat - (uint32_t)row * cpr;
+        } else {
+            row = flat / cpr;
+            c = (uint32_t)(flat - row * cpr);
+        }
+    }
+    LYTH_D void step(uint32_t rows, uint32_t chunks, uint32_t cpr) {
         row += rows;
         c += chunks;
         if (c >= cpr) { c -= cpr; row++; }
     }
 };
+struct MxFlat {
+    uint64_t rows, ld;
+    uint32_t cols, cpr;             // chunks per row
+    uint32_t step_rows, step_c;     // kMxThreads chunks on
+    bool narrow;                    // every flat index fits 32 bits
+};
 
-template <int FMT, int TY>
+// U: chunks of a thread, all loaded before the first is used.
+template <int FMT, int TY, bool VEC, int U>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_quantize_kernel(const typename MxElem<TY>::type *__restrict__ x, uint64_t rows, uint32_t cols, uint64_t ldx,
-                       uint32_t cpr, bool vec, float inv6g, float g, uint8_t *__restrict__ codes,
-                       uint8_t *__restrict__ scales) {
-    const uint64_t total = rows * cpr, stride = (uint64_t)gridDim.x * kMxThreads;
-    const uint64_t step_rows = stride / cpr;
-    const uint32_t step_c = (uint32_t)(stride % cpr);
-    const uint32_t words = cpr * 8 / Mx<FMT>::kWord;
-    const uint64_t row_bytes = (uint64_t)cpr * Mx<FMT>::kBits;
-    uint64_t flat = (uint64_t)blockIdx.x * kMxThreads + threadIdx.x;
-    MxWalk w(flat, cpr);
-    // whole warps: the warp's first chunk decides, the last warp's spare lanes hold zeros
-    for (uint64_t base = flat - (threadIdx.x & 31); base < total; base += stride) {
-        const bool live = w.row < rows;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (live) mx_load8<TY>(x + w.row * ldx, 8 * w.c, cols, vec, v);
-        mx_quantize8<FMT>(v, live, w.c, codes + w.row * row_bytes, scales + mx_scale_row(w.row, words), inv6g, g);
-        w.step(step_rows, step_c, cpr);
+    mx_quantize_kernel(const typename MxElem<TY>::type *__restrict__ x, MxFlat f, float inv6g, float g,
+                       uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    const uint32_t words = f.cpr * 16 / Mx<FMT>::kWord;
+    const uint64_t row_bytes = (uint64_t)f.cpr * 2 * Mx<FMT>::kBits;
+    const void *hi = x + (f.rows - 1) * f.ld + f.cols;
+    MxWalk w((uint64_t)blockIdx.x * (kMxThreads * U) + threadIdx.x, f.cpr, f.narrow);
+    uint64_t row[U];
+    uint32_t c[U], in[U][kMxWords<TY>];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        row[u] = w.row;
+        c[u] = w.c;
+        if (w.row < f.rows) {
+            mx_load<TY, VEC>(x + w.row * f.ld, w.c, f.cols, x, hi, in[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kMxWords<TY>; i++) in[u][i] = 0;
+        }
+        w.step(f.step_rows, f.step_c, f.cpr);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float v[16];
+        mx_widen<TY>(in[u], v);
+        mx_quantize<FMT>(v, mx_top_words<TY>(in[u]), row[u] < f.rows, c[u], codes + row[u] * row_bytes,
+                         scales + mx_scale_row(row[u], words), inv6g, g);
     }
 }
 
-template <int FMT, int TY>
+template <int FMT, int TY, bool VEC, int U>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, uint64_t rows,
-                         uint32_t cols, uint64_t ldo, uint32_t cpr, bool vec, float g,
+    mx_dequantize_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxFlat f, float g,
                          typename MxElem<TY>::type *__restrict__ out) {
-    const uint64_t total = rows * cpr, stride = (uint64_t)gridDim.x * kMxThreads;
-    const uint64_t step_rows = stride / cpr;
-    const uint32_t step_c = (uint32_t)(stride % cpr);
-    const uint32_t words = cpr * 8 / Mx<FMT>::kWord;
-    uint64_t flat = (uint64_t)blockIdx.x * kMxThreads + threadIdx.x;
-    MxWalk w(flat, cpr);
-    for (; flat < total; flat += stride, w.step(step_rows, step_c, cpr)) {
-        if (8 * w.c >= cols) continue;
-        const uint8_t *at = codes + flat * Mx<FMT>::kBits;
-        uint32_t h[4];
+    const uint32_t words = f.cpr * 16 / Mx<FMT>::kWord;
+    constexpr int kLanes = Mx<FMT>::kBlock / 16, kW = Mx<FMT>::kBits / 2;  // lanes of a block, words of a chunk
+    const uint64_t flat = (uint64_t)blockIdx.x * (kMxThreads * U) + threadIdx.x;
+    MxWalk w(flat, f.cpr, f.narrow);
+    uint64_t row[U];
+    uint32_t c[U], in[U][kW], byte[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        row[u] = w.row;
+        c[u] = w.c;
+        byte[u] = 0;
+#pragma unroll
+        for (int i = 0; i < kW; i++) in[u][i] = 0;
+        if (w.row < f.rows) {
+            const uint8_t *at = codes + (flat + u * kMxThreads) * 4 * kW;
+            const uint32_t blk = w.c / kLanes;
+            byte[u] = scales[mx_scale_row(w.row, words) + (uint64_t)(blk / 4) * 512 + (blk & 3)];
+            if constexpr (FMT == LYTH_MX_FP8) {
+                const uint4 t = *reinterpret_cast<const uint4 *>(at);
+                in[u][0] = t.x; in[u][1] = t.y; in[u][2] = t.z; in[u][3] = t.w;
+            } else {
+                const uint2 t = *reinterpret_cast<const uint2 *>(at);
+                in[u][0] = t.x; in[u][1] = t.y;
+            }
+        }
+        w.step(f.step_rows, f.step_c, f.cpr);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        uint32_t h[8], o[kMxWords<TY>];
         if constexpr (FMT == LYTH_MX_FP8) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(at);
-            e4m3x4_f16(u.x, h[0], h[1]);
-            e4m3x4_f16(u.y, h[2], h[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) e4m3x4_f16(in[u][i], h[2 * i], h[2 * i + 1]);
         } else {
-            e2m1x8_f16(*reinterpret_cast<const uint32_t *>(at), h);
-        }
-        constexpr int kLanes = Mx<FMT>::kBlock / 8;
-        const uint32_t blk = w.c / kLanes;
-        const uint8_t byte = scales[mx_scale_row(w.row, words) + (uint64_t)(blk / 4) * 512 + (blk & 3)];
-        const float s = mx_scales2<FMT>(byte).x;
-        float v[8];
+            uint32_t a[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = f16x2_f32(h[i]);
-            v[2 * i] = __fmul_rn(f.x, s);
-            v[2 * i + 1] = __fmul_rn(f.y, s);
-        }
-        if constexpr (FMT == LYTH_MX_NVFP4) {
+            for (int i = 0; i < 2; i++) {
+                e2m1x8_f16(in[u][i], a);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], g);
+                for (int j = 0; j < 4; j++) h[4 * i + j] = a[j];
+            }
         }
-        mx_store8<TY>(out + w.row * ldo, 8 * w.c, cols, vec, v);
+        const float s = mx_scales2<FMT>(byte[u]).x;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float2 t = mx_mul2(f16x2_f32(h[i]), make_float2(s, s));
+            if constexpr (FMT == LYTH_MX_NVFP4) t = mx_mul2(t, make_float2(g, g));
+            v[2 * i] = t.x;
+            v[2 * i + 1] = t.y;
+        }
+        mx_narrow<TY>(v, o);
+        mx_store<TY, VEC>(out + row[u] * f.ld, c[u], f.cols, row[u] < f.rows, o);
     }
 }
 
@@ -93,58 +137,84 @@ __global__ void __launch_bounds__(kMxThreads)
 //
 // blockDim.x threads (whole warps) own a row, blockDim.y rows share a block. V > 0: a thread's V
 // chunks of h stay in registers between the sum and the scaling, so a row is read once. V = 0
-// (rows wider than 1024 threads x 4 chunks): the second pass reads x and the residual again, and
+// (rows wider than 1024 threads x 2 chunks): the second pass reads x and the residual again, and
 // writes residual_out only then, since it may be either of them.
-template <int FMT, int TY, int V>
+template <int FMT, int TY, int V, bool VEC>
 __global__ void __launch_bounds__(1024)
     mx_rmsnorm_kernel(const typename MxElem<TY>::type *x, const typename MxElem<TY>::type *residual,
                       typename MxElem<TY>::type *residual_out, const typename MxElem<TY>::type *__restrict__ weight,
-                      uint64_t rows, uint32_t cols, uint64_t ldx, uint64_t ldr, uint64_t ldo, uint32_t cpr, bool vec,
-                      float eps, float inv6g, float g, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+                      uint64_t rows, uint32_t cols, uint64_t ldx, uint64_t ldr, uint64_t ldo, uint32_t cpr, float eps,
+                      float inv6g, float g, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    constexpr int N = kMxWords<TY>, kHeld = V > 0 ? V : 1;
     __shared__ float part[32];
     const uint32_t tpr = blockDim.x, warps = tpr >> 5;
-    const uint32_t words = cpr * 8 / Mx<FMT>::kWord;
-    const uint64_t row_bytes = (uint64_t)cpr * Mx<FMT>::kBits;
-    for (uint64_t row0 = (uint64_t)blockIdx.x * blockDim.y; row0 < rows; row0 += (uint64_t)gridDim.x * blockDim.y) {
+    const uint32_t words = cpr * 16 / Mx<FMT>::kWord;
+    const uint64_t row_bytes = (uint64_t)cpr * 2 * Mx<FMT>::kBits, step = (uint64_t)gridDim.x * blockDim.y;
+    const void *x_hi = x + (rows - 1) * ldx + cols, *r_hi = residual ? residual + (rows - 1) * ldr + cols : nullptr;
+    auto load = [&](uint64_t row, uint32_t c, uint32_t (&a)[N], uint32_t (&b)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) a[i] = b[i] = 0;
+        if (row < rows && c < cpr) {
+            mx_load<TY, VEC>(x + row * ldx, c, cols, x, x_hi, a);
+            if (residual) mx_load<TY, VEC>(residual + row * ldr, c, cols, residual, r_hi, b);
+        }
+    };
+    auto add = [&](const uint32_t (&a)[N], const uint32_t (&b)[N], float (&v)[16]) {
+        mx_widen<TY>(a, v);
+        if (residual) {
+            float r[16];
+            mx_widen<TY>(b, r);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float2 t = mx_add2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(r[2 * i], r[2 * i + 1]));
+                v[2 * i] = t.x;
+                v[2 * i + 1] = t.y;
+            }
+        }
+    };
+    auto keep = [&](uint64_t row, uint32_t c, const float (&v)[16]) {
+        if (residual_out) {
+            uint32_t o[N];
+            mx_narrow<TY>(v, o);
+            mx_store<TY, VEC>(residual_out + row * ldo, c, cols, row < rows && c < cpr, o);
+        }
+    };
+    auto load_weight = [&](uint32_t c, uint32_t (&w)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = 0;
+        if (c < cpr) mx_load<TY, VEC>(weight, c, cols, weight, weight + cols, w);
+    };
+    uint64_t row0 = (uint64_t)blockIdx.x * blockDim.y;
+    for (; row0 < rows; row0 += step) {
         const uint64_t row = row0 + threadIdx.y;
-        const bool in = row < rows;
-        const typename MxElem<TY>::type *xr = x + row * ldx;
-        const typename MxElem<TY>::type *rr = residual ? residual + row * ldr : nullptr;
-        typename MxElem<TY>::type *ro = residual_out ? residual_out + row * ldo : nullptr;
         float ss = 0.0f;
-        float h[V > 0 ? V : 1][8];
-        auto sum8 = [&](uint32_t c, float (&v)[8], bool live) {
-            if (!live) {
+        float h[kHeld][16];
+        auto square = [&](const float (&v)[16]) {
+            float2 t = make_float2(ss, 0.0f);
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = 0.0f;
-                return;
+            for (int i = 0; i < 8; i++) {
+                const float2 u = make_float2(v[2 * i], v[2 * i + 1]);
+                t = mx_fma2(u, u, t);
             }
-            mx_load8<TY>(xr, 8 * c, cols, vec, v);
-            if (rr) {
-                float r[8];
-                mx_load8<TY>(rr, 8 * c, cols, vec, r);
-#pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = __fadd_rn(v[i], r[i]);
-            }
+            ss = __fadd_rn(t.x, t.y);
         };
+        uint32_t w[kHeld][N];
         if constexpr (V > 0) {
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const uint32_t c = threadIdx.x + j * tpr;
-                sum8(c, h[j], in && c < cpr);
-            }
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const uint32_t c = threadIdx.x + j * tpr;
-                if (ro && in && 8 * c < cols) mx_store8<TY>(ro, 8 * c, cols, vec, h[j]);
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = __fmaf_rn(h[j][i], h[j][i], ss);
+                uint32_t a[N], b[N];
+                load(row, threadIdx.x + j * tpr, a, b);
+                add(a, b, h[j]);
+                square(h[j]);
+                keep(row, threadIdx.x + j * tpr, h[j]);
+                load_weight(threadIdx.x + j * tpr, w[j]);
             }
         } else {
             for (uint32_t c = threadIdx.x; c < cpr; c += tpr) {
-                sum8(c, h[0], in);
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss = __fmaf_rn(h[0][i], h[0][i], ss);
+                uint32_t a[N], b[N];
+                load(row, c, a, b);
+                add(a, b, h[0]);
+                square(h[0]);
             }
         }
 #pragma unroll
@@ -159,26 +229,31 @@ __global__ void __launch_bounds__(1024)
         }
         const float scale = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)cols), eps));
         uint8_t *cr = codes + row * row_bytes, *sr = scales + mx_scale_row(row, words);
-        // whole warps walk the chunks (mx_quantize8 shuffles): the lanes behind the row hold zeros
+        // whole warps walk the chunks (mx_quantize shuffles); lanes behind the row store nothing, and
+        // share no block or scale word with lanes inside it
         const int trips = V > 0 ? V : (int)((cpr + tpr - 1) / tpr);
-#pragma unroll(V > 0 ? V : 1)
+#pragma unroll(kHeld)
         for (int j = 0; j < trips; j++) {
             const uint32_t c = threadIdx.x + (uint32_t)j * tpr;
-            const bool live = in && c < cpr;
-            float(&v)[8] = h[V > 0 ? j : 0];
+            const bool live = row < rows && c < cpr;
+            float(&v)[16] = h[V > 0 ? j : 0];
             if constexpr (V == 0) {
-                sum8(c, v, live);
-                if (ro && live && 8 * c < cols) mx_store8<TY>(ro, 8 * c, cols, vec, v);
+                uint32_t a[N], b[N];
+                load(row, c, a, b);
+                add(a, b, v);
+                keep(row, c, v);
             }
-            float wt[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (live) mx_load8<TY>(weight, 8 * c, cols, vec, wt);
+            if constexpr (V == 0) load_weight(c, w[0]);
+            float wt[16];
+            mx_widen<TY>(w[V > 0 ? j : 0], wt);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = live ? __fmul_rn(__fmul_rn(v[i], scale), wt[i]) : 0.0f;
-            // columns behind `cols` stay zero even where the row's sum is not a number
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (8 * c + i >= cols) v[i] = 0.0f;
-            mx_quantize8<FMT>(v, live, c, cr, sr, inv6g, g);
+            for (int i = 0; i < 8; i++) {
+                const float2 y = mx_mul2(mx_mul2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(scale, scale)),
+                                         make_float2(wt[2 * i], wt[2 * i + 1]));
+                v[2 * i] = y.x;
+                v[2 * i + 1] = y.y;
+            }
+            mx_quantize<FMT>(v, mx_top(v), live, c, cr, sr, inv6g, g);
         }
     }
 }
@@ -193,6 +268,21 @@ extern "C" uint64_t lyth_b200_mx_row_bytes(int fmt, uint32_t cols) {
 
 extern "C" uint64_t lyth_b200_mx_scale_bytes(int fmt, uint64_t rows, uint32_t cols) {
     return mx_known(fmt) ? (rows + 127) / 128 * (mx_padded(fmt, cols) / (4 * mx_block(fmt))) * 512 : 0;
+}
+
+// Chunks to blocks of kMxThreads * u; grid 0 where they do not fit one launch.
+static MxFlat mx_flat(int fmt, uint64_t rows, uint32_t cols, uint64_t ld, int u, unsigned &grid) {
+    MxFlat f;
+    f.rows = rows;
+    f.ld = ld;
+    f.cols = cols;
+    f.cpr = (uint32_t)(mx_padded(fmt, cols) / kMxChunk);
+    f.step_rows = kMxThreads / f.cpr;
+    f.step_c = kMxThreads % f.cpr;
+    const uint64_t per = (uint64_t)kMxThreads * u, blocks = (rows * f.cpr + per - 1) / per;
+    f.narrow = blocks * per <= 0xFFFFFFFFull;
+    grid = blocks < (1ull << 31) ? (unsigned)blocks : 0u;
+    return f;
 }
 
 // What every entry here asks of its sizes: known format and type, columns that a 32-bit index
@@ -212,13 +302,14 @@ extern "C" int lyth_b200_quantize_mx(int fmt, int ty, uint64_t rows, uint32_t co
     if (rows == 0) return LYTH_OK;
     if (!x || !codes || !scales) return LYTH_E_INVALID;
     if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
-    const uint32_t cpr = (uint32_t)(mx_padded(fmt, cols) / 8);
-    const bool vec = aligned16(x) && ldx * mx_ty_bytes(ty) % 16 == 0;
-    const unsigned grid = stream_grid(rows * cpr, kMxThreads);
+    const bool vec = cols % 16 == 0 && aligned32(x) && ldx * mx_ty_bytes(ty) % 32 == 0;
+    unsigned grid;
+    const MxFlat f = mx_flat(fmt, rows, cols, ldx, vec ? 2 : 1, grid);
+    if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
-                     mx_quantize_kernel<FMT, TY><<<grid, kMxThreads, 0, s>>>(
-                         static_cast<const MxElem<TY>::type *>(x), rows, cols, ldx, cpr, vec, inv6g, tensor_scale,
-                         codes, scales));
+                     auto k = vec ? mx_quantize_kernel<FMT, TY, true, 2> : mx_quantize_kernel<FMT, TY, false, 1>;
+                     k<<<grid, kMxThreads, 0, s>>>(static_cast<const MxElem<TY>::type *>(x), f, inv6g, tensor_scale,
+                                                   codes, scales));
     return last_launch_status();
 }
 
@@ -232,35 +323,38 @@ extern "C" int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t 
     if (rows == 0) return LYTH_OK;
     if (!out || !codes || !scales) return LYTH_E_INVALID;
     if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
-    const uint32_t cpr = (uint32_t)(mx_padded(fmt, cols) / 8);
-    const bool vec = aligned16(out) && ldo * mx_ty_bytes(ty) % 16 == 0;
-    const unsigned grid = stream_grid(rows * cpr, kMxThreads);
+    const bool vec = cols % 16 == 0 && aligned32(out) && ldo * mx_ty_bytes(ty) % 32 == 0;
+    unsigned grid;
+    const MxFlat f = mx_flat(fmt, rows, cols, ldo, vec ? 2 : 1, grid);
+    if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
-                     mx_dequantize_kernel<FMT, TY><<<grid, kMxThreads, 0, s>>>(
-                         codes, scales, rows, cols, ldo, cpr, vec, tensor_scale, static_cast<MxElem<TY>::type *>(out)));
+                     auto k = vec ? mx_dequantize_kernel<FMT, TY, true, 2> : mx_dequantize_kernel<FMT, TY, false, 1>;
+                     k<<<grid, kMxThreads, 0, s>>>(codes, scales, f, tensor_scale, static_cast<MxElem<TY>::type *>(out)));
     return last_launch_status();
 }
 
 template <int FMT, int TY>
-static void rmsnorm_launch(const void *x, const void *residual, void *residual_out, const void *weight, uint64_t rows,
+static int rmsnorm_launch(const void *x, const void *residual, void *residual_out, const void *weight, uint64_t rows,
                            uint32_t cols, uint64_t ldx, uint64_t ldr, uint64_t ldo, uint32_t cpr, bool vec, float eps,
                            float inv6g, float g, uint8_t *codes, uint8_t *scales, cudaStream_t s) {
     using T = typename MxElem<TY>::type;
     const T *xt = static_cast<const T *>(x), *rt = static_cast<const T *>(residual), *wt = static_cast<const T *>(weight);
     T *ot = static_cast<T *>(residual_out);
-    const int v = cpr <= 1024 ? 1 : cpr <= 4096 ? 4 : 0;
-    uint32_t tpr = v ? ((cpr + v - 1) / v + 31) / 32 * 32 : 1024;
-    const uint32_t per = tpr < 256 ? 256 / tpr : 1;
+    // One chunk a thread is quickest for few rows (one 4096-wide bf16 row: 2.6 us, two chunks 2.9); two
+    // chunks in blocks half as large carry more bytes in flight once the rows fill the machine (8192
+    // rows: 39.1 against 42.1 us). Of f32 and of rows in shifted words two would spill.
+    const bool many = TY != 0 && vec && cpr >= 128 && rows >= 4ull * device_sms();
+    const int v = cpr <= 1024 && !many ? 1 : cpr <= 2048 ? 2 : 0;
+    const uint32_t tpr = v ? ((cpr + v - 1) / v + 31) / 32 * 32 : 1024;
+    const uint32_t per = tpr < 128 ? 128 / tpr : 1;
     const dim3 block(tpr, per);
     const uint64_t need = (rows + per - 1) / per;
     const unsigned grid = need < (1u << 30) ? (unsigned)need : (1u << 30);
-#define LYTH_MX_NORM(V)                                                                                            \
-    mx_rmsnorm_kernel<FMT, TY, V><<<grid, block, 0, s>>>(xt, rt, ot, wt, rows, cols, ldx, ldr, ldo, cpr, vec, eps, \
-                                                         inv6g, g, codes, scales)
-    if (v == 1) LYTH_MX_NORM(1);
-    else if (v == 4) LYTH_MX_NORM(4);
-    else LYTH_MX_NORM(0);
-#undef LYTH_MX_NORM
+    auto k = v == 1   ? (vec ? mx_rmsnorm_kernel<FMT, TY, 1, true> : mx_rmsnorm_kernel<FMT, TY, 1, false>)
+             : v == 2 ? (vec ? mx_rmsnorm_kernel<FMT, TY, 2, true> : mx_rmsnorm_kernel<FMT, TY, 2, false>)
+                      : (vec ? mx_rmsnorm_kernel<FMT, TY, 0, true> : mx_rmsnorm_kernel<FMT, TY, 0, false>);
+    k<<<grid, block, 0, s>>>(xt, rt, ot, wt, rows, cols, ldx, ldr, ldo, cpr, eps, inv6g, g, codes, scales);
+    return last_launch_status();
 }
 
 extern "C" int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const void *x, uint64_t ldx,
@@ -276,13 +370,13 @@ extern "C" int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t col
     if (rows == 0) return LYTH_OK;
     if (!x || !weight || !codes || !scales) return LYTH_E_INVALID;
     if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
-    const uint32_t cpr = (uint32_t)(mx_padded(fmt, cols) / 8);
+    const uint32_t cpr = (uint32_t)(mx_padded(fmt, cols) / kMxChunk);
     const uint64_t size = mx_ty_bytes(ty);
-    const bool vec = aligned16(x) && ldx * size % 16 == 0 && aligned16(weight) &&
-                     (!residual || (aligned16(residual) && ldr * size % 16 == 0)) &&
-                     (!residual_out || (aligned16(residual_out) && ldo * size % 16 == 0));
+    const bool vec = cols % 16 == 0 && aligned32(x) && ldx * size % 32 == 0 && aligned32(weight) &&
+                     (!residual || (aligned32(residual) && ldr * size % 32 == 0)) &&
+                     (!residual_out || (aligned32(residual_out) && ldo * size % 32 == 0));
     LYTH_MX_DISPATCH(fmt, ty,
-                     rmsnorm_launch<FMT, TY>(x, residual, residual_out, weight, rows, cols, ldx, ldr, ldo, cpr, vec,
-                                             eps, inv6g, tensor_scale, codes, scales, s));
-    return last_launch_status();
+                     return (rmsnorm_launch<FMT, TY>(x, residual, residual_out, weight, rows, cols, ldx, ldr, ldo, cpr,
+                                                     vec, eps, inv6g, tensor_scale, codes, scales, s)));
+    return LYTH_E_UNSUPPORTED;
 }

@@ -138,7 +138,7 @@ def norm_ref(x, r, w, eps):
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("rows,cols,residual", [(1, 4096, True), (3, 1, True), (5, 100, False), (130, 777, True), (9, 8200, True),
-                                                (4, 33000, True), (2, 70001, False)])
+                                                (4, 33000, True), (2, 70001, False), (1300, 2048, True), (2600, 512, False)])
 def test_rmsnorm(cuda, fmt, ty, rows, cols, residual):
     gen = torch.Generator().manual_seed(rows * 31 + cols)
     x = torch.randn(rows, cols, generator=gen).to(ty).to(cuda)
