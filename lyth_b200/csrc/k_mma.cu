@@ -541,11 +541,13 @@ extern "C" int lyth_b200_device_error(void) {
     const int probe = probe_take_device_error();
     const int tx = transpose_take_device_error();
     const int mx = mx_take_device_error();
+    const int xv = xv_take_device_error();
     if (fused != LYTH_OK) return fused;
     if (gemv != LYTH_OK) return gemv;
     if (probe != LYTH_OK) return probe;
     if (tx != LYTH_OK) return tx;
     if (mx != LYTH_OK) return mx;
+    if (xv != LYTH_OK) return xv;
     int v = 0;
     cudaError_t e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int));
     if (e != cudaSuccess) return status_of(e);

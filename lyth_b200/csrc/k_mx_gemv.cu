@@ -10,14 +10,52 @@
 // that block's scale in f32 afterwards: four multiply-adds for the 64 codes a lane holds. Tensor-core
 // work is four times what the product needs and is idle capacity here.
 //
-// Range: bf16 x is brought into f16 by one power of two for all of x in the block (its largest finite
-// exponent to 2^14), undone in f32 at the end. Values below 2^-38 of the largest lose bits, which is
-// below the rounding of the f32 sum; every other bf16 value keeps all its bits.
+// What bounds the arithmetic is the conversion of codes (two codes an instruction, at half the issue
+// rate), so everything around it is kept off the warps that convert: one block per SM, in roles:
+//   producers (4 warps)  bring a stage -- 16 rows of W, up to 2048 bytes of each, and their scale words --
+//                        into a ring of shared-memory stages, four rows a warp: a bulk copy per row (one
+//                        lane each) and 16-byte asynchronous copies of the scales, completion on an
+//                        mbarrier. (One warp for all sixteen rows needed 2000 cycles to issue a stage.)
+//   consumers (16 warps) put x into shared memory as f16 once. Two teams of eight then take every other
+//                        16-row group, a warp every eighth 64-byte step of a stage, so that one team's
+//                        waits and sums lie under the other's conversions (all sixteen on one stage:
+//                        11.5 us). The partial sums of a group stay in shared memory, where all meet once
+//                        at the end and add them up in a fixed order. Where x does not fit, k is walked
+//                        in chunks, x staged chunk by chunk.
+// Every mbarrier wait is bounded (mbar.cuh); one that runs out sets the device error flag and the
+// block winds down. Loading and converting in the same warps, with four steps of loads in flight in
+// registers, took 13.2 us for one token through 14336 x 4096 NVFP4 weights: 9.5 us without the loads,
+// 10.6 us without the arithmetic.
+//
+// Range: bf16 x is brought into f16 by one power of two for all of x (its largest finite exponent to
+// 2^14), undone in f32 at the end. Values below 2^-38 of the largest lose bits, which is below the
+// rounding of the f32 sum; every other bf16 value keeps all its bits.
+#include "mbar.cuh"
 #include "mx.cuh"
 
 namespace lyth {
 
-constexpr int XV_WARPS = 8, XV_THREADS = 32 * XV_WARPS, XV_ROWS = 16;
+__device__ int g_xv_error = 0;
+
+constexpr int XV_WARPS = 16;                        // consumers
+constexpr int XV_TEAM = XV_WARPS / 2;               // a team takes every other group
+constexpr int XV_PRODUCERS = 4;                     // warps, one per quad of a group
+constexpr int XV_THREADS = 32 * (XV_WARPS + XV_PRODUCERS);
+constexpr int XV_SEG = 2048;                        // bytes of a row in a stage
+constexpr int XV_ROW = XV_SEG + 64;                 // their pitch: eight rows read at once hit all banks
+constexpr int XV_STEPS = XV_SEG / 64;               // steps in a whole stage
+constexpr int XV_W_BYTES = 16 * XV_ROW;
+
+// Groups whose partial sums are kept before they are added up: all of a block's, up to this many.
+template <int PAIRS>
+constexpr int kXvBatch = PAIRS == 4 ? 4 : 8;
+
+// Scale words of a row in a stage: one for 64 (E4M3: 128) bytes of MX codes, two for 64 of NVFP4.
+template <int FMT>
+struct Xv {
+    static constexpr int kWords = FMT == LYTH_MX_FP8 ? XV_STEPS / 2 : FMT == LYTH_MX_FP4 ? XV_STEPS : 2 * XV_STEPS;
+    static constexpr int kStage = XV_W_BYTES + kWords * 64;  // a quad's four words are 16 bytes
+};
 
 struct XvArgs {
     const void *x;
@@ -25,11 +63,13 @@ struct XvArgs {
     void *y;
     uint64_t ldx, ldy;
     uint32_t m, n, cols;
-    uint32_t row_bytes, words;  // bytes of a row of codes; scale words along k
-    uint32_t iters;             // steps of 64 bytes along k
-    uint32_t chunk;             // steps whose x is in shared memory at once
+    uint32_t quads_each, quads_more;  // quads of a block; blocks that have one more
+    uint32_t row_bytes, words;        // bytes of a row of codes; scale words along k
+    uint32_t segs;                    // stages along k
+    uint32_t chunk;                   // segments whose x is in shared memory at once
+    uint32_t stages;                  // of the ring
     float alpha;
-    bool vec;                   // rows of x start on 16 bytes
+    bool vec;                         // rows of x start on 16 bytes
 };
 
 LYTH_D void xv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -38,178 +78,373 @@ LYTH_D void xv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of codes as pairs of f16 in k order: 16 registers of E2M1, 8 of E4M3.
+// 16 bytes of shared memory where `on`, else v as it was.
+LYTH_D void xv_load_x(uint4 &v, uint32_t at, bool on) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+                 : "r"(at), "r"((uint32_t)on)
+                 : "memory");
+}
+
+// The eight codes of unit j of 16 bytes as four pairs of f16, in k order.
 template <int FMT>
-LYTH_D void xv_decode(const uint4 &u, uint32_t (&h)[FMT == LYTH_MX_FP8 ? 8 : 16]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (FMT == LYTH_MX_FP8) {
-            e4m3x4_f16(w[i], h[2 * i], h[2 * i + 1]);
-        } else {
-            uint32_t q[4];
-            e2m1x8_f16(w[i], q);
-#pragma unroll
-            for (int j = 0; j < 4; j++) h[4 * i + j] = q[j];
-        }
+LYTH_D void xv_decode(const uint4 &u, int j, uint32_t (&h)[4]) {
+    if constexpr (FMT == LYTH_MX_FP8) {
+        e4m3x4_f16(j == 0 ? u.x : u.z, h[0], h[1]);
+        e4m3x4_f16(j == 0 ? u.y : u.w, h[2], h[3]);
+    } else {
+        e2m1x8_f16(j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w, h);
     }
 }
 
-// Row i (0..15) of tile t: four neighbouring rows of each 32-row quarter of a scale tile, whose
-// sixteen scale words are contiguous.
-LYTH_D uint64_t xv_row(uint64_t t, uint32_t i) { return (t >> 3) * 128 + (i & 3) * 32 + (t & 7) * 4 + (i >> 2); }
-
-// PAIRS: token pairs (1, 2 or 4).
-template <int FMT, int TY, int PAIRS>
-__global__ void __launch_bounds__(XV_THREADS) mx_gemv_kernel(XvArgs p) {
-    using T = typename MxElem<TY>::type;
-    constexpr int kCodes = FMT == LYTH_MX_FP8 ? 16 : 32;  // codes of a lane per step
-    constexpr int kStep = 4 * kCodes;                     // columns of a step
-    constexpr int kUnits = kCodes / 8;                    // 16-byte units of f16 x of a lane per step
-    extern __shared__ uint4 sx[];                         // [2 PAIRS][chunk][4 lanes][kUnits]
-    __shared__ float s_part[XV_WARPS][2 * PAIRS][XV_ROWS];
-    __shared__ uint32_t s_max[XV_WARPS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t units = p.chunk * 4 * kUnits;          // per token
-
-    // x to shared memory as f16. Units are stored with their low bits exchanged (lane of the quad,
-    // token) so that the eight lanes reading at once reach eight different 16-byte columns.
-    float unscale = 1.0f;
-    float scale = 1.0f;
-    if constexpr (TY == LYTH_NARROW_BF16) {
-        uint32_t top = 0;
-        const uint32_t all = (p.cols + 7) / 8;
-        for (uint64_t i = threadIdx.x; i < (uint64_t)p.m * all; i += XV_THREADS) {
-            float v[8];
-            mx_load8<TY>(static_cast<const T *>(p.x) + i / all * p.ldx, 8 * (uint32_t)(i % all), p.cols, p.vec, v);
+// Eight values of x as four words of 16-bit pairs, zero behind `cols`.
+template <int TY>
+LYTH_D uint4 xv_load8(const typename MxElem<TY>::type *row, uint32_t col, uint32_t cols, bool vec) {
+    if (vec && col + 8 <= cols) return *reinterpret_cast<const uint4 *>(row + col);
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
+    uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t e = (__float_as_uint(v[j]) >> 23) & 0xFFu;
-                if (e < 255u) top = max(top, e);
-            }
-        }
-        top = __reduce_max_sync(0xFFFFFFFFu, top);
-        if (lane == 0) s_max[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < XV_WARPS; i++) top = max(top, s_max[i]);
-        // 2^(14 - e) and its inverse, e the largest exponent; kept within normal f32 numbers
-        const int e = (int)top - 127, sh = min(14 - e, 126);
-        scale = __uint_as_float((uint32_t)(sh + 127) << 23);
-        unscale = __uint_as_float((uint32_t)(127 - sh) << 23);
+    for (int i = 0; i < 4; i++) {
+        const uint32_t c = col + 2 * i, a = c < cols ? h[c] : 0u, b = c + 1 < cols ? h[c + 1] : 0u;
+        w[i] = a | b << 16;
     }
-    const uint64_t tile = blockIdx.x;
-    const uint64_t r0 = xv_row(tile, g), r1 = xv_row(tile, g + 8);
-    const bool in0 = r0 < p.n, in1 = r1 < p.n;
-    const uint8_t *w0 = p.w + r0 * p.row_bytes + 16 * t, *w1 = p.w + r1 * p.row_bytes + 16 * t;
-    const uint8_t *s0 = p.s + mx_scale_row(r0, p.words), *s1 = p.s + mx_scale_row(r1, p.words);
-    const bool mine = (g & 3) == t;  // this lane's x columns: token g / 4 of each pair
-    float acc[PAIRS][2] = {};
-    for (uint32_t c0 = 0; c0 < p.iters; c0 += p.chunk) {
-        if (c0) __syncthreads();
-        for (uint32_t i = threadIdx.x; i < 2 * PAIRS * units; i += XV_THREADS) {
-            const uint32_t tok = i / units, u = i % units, l = (u / kUnits) & 3;
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (tok < p.m) mx_load8<TY>(static_cast<const T *>(p.x) + tok * p.ldx, 8 * (c0 * 4 * kUnits + u), p.cols, p.vec, v);
-    #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = __fmul_rn(v[j], scale);
-            const uint32_t sw = (kUnits == 4 ? l : 0u) ^ (tok & 1);
-            sx[tok * units + (u ^ sw)] = make_uint4(mx_pack2<LYTH_NARROW_F16>(v[0], v[1]), mx_pack2<LYTH_NARROW_F16>(v[2], v[3]),
-                                                    mx_pack2<LYTH_NARROW_F16>(v[4], v[5]), mx_pack2<LYTH_NARROW_F16>(v[6], v[7]));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The largest exponent field among eight bf16 values that are numbers.
+LYTH_D uint32_t xv_top(uint4 u) {
+    const uint32_t a = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+    uint32_t top = max(a & 0xFFFFu, a >> 16) >> 7;
+    if (top == 255u) {  // an infinity or a NaN among them: look at each
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        top = 0;
+        for (int i = 0; i < 4; i++) {
+            const uint32_t lo = (w[i] >> 7) & 0xFFu, hi = (w[i] >> 23) & 0xFFu;
+            if (lo < 255u) top = max(top, lo);
+            if (hi < 255u) top = max(top, hi);
         }
-        __syncthreads();
-    const uint32_t c1 = min(c0 + p.chunk, p.iters);
-    for (uint32_t it = c0 + warp; it < c1; it += XV_WARPS) {
-        const bool ink = it * 64 + 16 * t < p.row_bytes;
-        uint4 u0 = make_uint4(0, 0, 0, 0), u1 = u0;
-        if (in0 && ink) u0 = __ldcs(reinterpret_cast<const uint4 *>(w0 + (uint64_t)it * 64));
-        if (in1 && ink) u1 = __ldcs(reinterpret_cast<const uint4 *>(w1 + (uint64_t)it * 64));
+    }
+    return top;
+}
+// Eight values in f16: f16 as they are, bf16 times a power of two.
+template <int TY>
+LYTH_D uint4 xv_f16(uint4 u, float scale) {
+    if constexpr (TY == LYTH_NARROW_F16) {
+        return u;
+    } else {
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = mx_mul2(mx_unpack2<TY>(w[i]), make_float2(scale, scale));
+            w[i] = mx_pack2<LYTH_NARROW_F16>(f.x, f.y);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+LYTH_D void xv_sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * XV_WARPS) : "memory"); }
+LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, &g_xv_error); }
+
+// Where a block is in its walk: batches of groups, chunks of k, groups, segments. All roles take the
+// same steps.
+struct XvWalk {
+    uint64_t tile0;          // first scale tile (128 rows) of the batch; rows and quads count from it
+    uint32_t lo, hi, last;   // the batch's quads, and the last row of W
+    uint32_t groups;         // of the batch
+};
+template <int BATCH>
+LYTH_D bool xv_batch(const XvArgs &p, uint32_t index, XvWalk &w) {
+    const uint64_t q_lo = (uint64_t)blockIdx.x * p.quads_each + min(blockIdx.x, p.quads_more);
+    const uint64_t q_hi = q_lo + p.quads_each + (blockIdx.x < p.quads_more ? 1 : 0);
+    const uint64_t b_lo = q_lo + (uint64_t)index * (4 * BATCH);
+    if (b_lo >= q_hi) return false;
+    w.tile0 = b_lo >> 5;
+    w.lo = (uint32_t)b_lo & 31u;
+    w.hi = w.lo + (uint32_t)min(q_hi - b_lo, (uint64_t)(4 * BATCH));
+    w.last = (uint32_t)min((uint64_t)p.n - 1 - w.tile0 * 128, (uint64_t)511);
+    w.groups = (w.hi - w.lo + 3) / 4;
+    return true;
+}
+LYTH_D uint32_t xv_row(uint32_t quad, uint32_t j) { return (quad >> 5) * 128 + (quad & 31) + 32 * j; }
+
+// U steps (it, it + XV_TEAM, ..) of a warp in the stage at `at`, independent of one another until
+// their sums meet in acc: acc[pair][row g, row g + 8] of token t / 2 of the pair. `words`: scale words
+// that the row still has from the stage on. x_off: of step `it` in shared x, bytes.
+template <int FMT, int PAIRS, int U>
+LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_off, uint32_t g, uint32_t t, bool mine,
+                     const uint32_t (&x_at)[PAIRS], uint32_t words, uint4 (&xb)[4],
+                     float (&acc)[PAIRS][2]) {
+    constexpr int kUnits = FMT == LYTH_MX_FP8 ? 2 : 4, kSub = FMT == LYTH_MX_NVFP4 ? 2 : 1;
+    uint4 u0[U], u1[U];
+    uint32_t q0[U], q1[U];
+    float cc[U][PAIRS][kSub][4] = {};
+#pragma unroll
+    for (int s = 0; s < U; s++) {
+        const uint32_t i = it + s * XV_TEAM;
+        u0[s] = *reinterpret_cast<const uint4 *>(at + g * XV_ROW + i * 64 + t * 16);
+        u1[s] = *reinterpret_cast<const uint4 *>(at + (g + 8) * XV_ROW + i * 64 + t * 16);
         // the scale word that holds this lane's two columns' blocks
-        const uint32_t word = FMT == LYTH_MX_FP8 ? it >> 1 : FMT == LYTH_MX_FP4 ? it : 2 * it + (t & 1);
-        uint32_t q0 = 0, q1 = 0;
-        if (word < p.words) {
-            if (in0) q0 = *reinterpret_cast<const uint32_t *>(s0 + (uint64_t)word * 512);
-            if (in1) q1 = *reinterpret_cast<const uint32_t *>(s1 + (uint64_t)word * 512);
-        }
-        uint32_t h0[kCodes / 2], h1[kCodes / 2];
-        xv_decode<FMT>(u0, h0);
-        xv_decode<FMT>(u1, h1);
+        const uint32_t word = FMT == LYTH_MX_FP8 ? i >> 1 : FMT == LYTH_MX_FP4 ? i : 2 * i + (t & 1);
+        q0[s] = *reinterpret_cast<const uint32_t *>(at + XV_W_BYTES + word * 64 + g * 4);
+        q1[s] = *reinterpret_cast<const uint32_t *>(at + XV_W_BYTES + word * 64 + g * 4 + 32);
+        if (FMT == LYTH_MX_NVFP4 && word >= words) q0[s] = q1[s] = 0;  // a row may end in half a step
+    }
 #pragma unroll
-        for (int pr = 0; pr < PAIRS; pr++) {
-            uint32_t b[kCodes / 2];
-            const uint32_t tok = 2 * pr + (g >> 2);
+    for (int j = 0; j < kUnits; j++) {
 #pragma unroll
-            for (int j = 0; j < kUnits; j++) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (mine) v = sx[tok * units + ((((it - c0) * 4 + t) * kUnits + j) ^ ((kUnits == 4 ? t : 0) ^ (tok & 1)))];
-                b[4 * j] = v.x; b[4 * j + 1] = v.y; b[4 * j + 2] = v.z; b[4 * j + 3] = v.w;
-            }
-            constexpr int kSub = FMT == LYTH_MX_NVFP4 ? 2 : 1;  // scale blocks of a lane per step
-            float c[kSub][4] = {};
+        for (int s = 0; s < U; s++) {
+            uint32_t h0[4], h1[4];
+            xv_decode<FMT>(u0[s], j, h0);
+            xv_decode<FMT>(u1[s], j, h1);
 #pragma unroll
-            for (int j = 0; j < kCodes / 4; j++)
-                xv_mma(c[j * kSub / (kCodes / 4)], h0[2 * j], h1[2 * j], h0[2 * j + 1], h1[2 * j + 1], b[2 * j], b[2 * j + 1]);
-            // columns 2t, 2t + 1: token t / 2 of the pair, quad lanes 2 (t % 2) and the next
-            if constexpr (FMT == LYTH_MX_NVFP4) {
-                const float2 a0 = mx_scales2<FMT>(q0), a1 = mx_scales2<FMT>(q0 >> 16);
-                const float2 b0 = mx_scales2<FMT>(q1), b1 = mx_scales2<FMT>(q1 >> 16);
-                acc[pr][0] = __fmaf_rn(c[0][0], a0.x, acc[pr][0]);
-                acc[pr][0] = __fmaf_rn(c[1][0], a0.y, acc[pr][0]);
-                acc[pr][0] = __fmaf_rn(c[0][1], a1.x, acc[pr][0]);
-                acc[pr][0] = __fmaf_rn(c[1][1], a1.y, acc[pr][0]);
-                acc[pr][1] = __fmaf_rn(c[0][2], b0.x, acc[pr][1]);
-                acc[pr][1] = __fmaf_rn(c[1][2], b0.y, acc[pr][1]);
-                acc[pr][1] = __fmaf_rn(c[0][3], b1.x, acc[pr][1]);
-                acc[pr][1] = __fmaf_rn(c[1][3], b1.y, acc[pr][1]);
-            } else if constexpr (FMT == LYTH_MX_FP4) {
-                const float2 a = mx_scales2<FMT>(q0 >> (16 * (t & 1))), bb = mx_scales2<FMT>(q1 >> (16 * (t & 1)));
-                acc[pr][0] = __fmaf_rn(c[0][0], a.x, acc[pr][0]);
-                acc[pr][0] = __fmaf_rn(c[0][1], a.y, acc[pr][0]);
-                acc[pr][1] = __fmaf_rn(c[0][2], bb.x, acc[pr][1]);
-                acc[pr][1] = __fmaf_rn(c[0][3], bb.y, acc[pr][1]);
-            } else {
-                const uint32_t sh = 16 * (it & 1) + 8 * (t & 1);  // both columns in one block of 32
-                const float a = mx_scales2<FMT>((q0 >> sh) & 0xFFu).x, bb = mx_scales2<FMT>((q1 >> sh) & 0xFFu).x;
-                acc[pr][0] = __fmaf_rn(c[0][0], a, acc[pr][0]);
-                acc[pr][0] = __fmaf_rn(c[0][1], a, acc[pr][0]);
-                acc[pr][1] = __fmaf_rn(c[0][2], bb, acc[pr][1]);
-                acc[pr][1] = __fmaf_rn(c[0][3], bb, acc[pr][1]);
+            for (int pr = 0; pr < PAIRS; pr++) {
+                uint4 &v = xb[(s * PAIRS + pr) % 4];
+                xv_load_x(v, x_at[pr] + x_off + s * (XV_TEAM * 4 * kUnits * 16) + 64 * j, mine);
+                xv_mma(cc[s][pr][j * kSub / kUnits], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
+                xv_mma(cc[s][pr][j * kSub / kUnits], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
             }
         }
     }
-    }
 #pragma unroll
-    for (int pr = 0; pr < PAIRS; pr++)
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            acc[pr][i] = __fadd_rn(acc[pr][i], __shfl_xor_sync(0xFFFFFFFFu, acc[pr][i], 1));
-            if ((t & 1) == 0) s_part[warp][2 * pr + (t >> 1)][g + 8 * i] = acc[pr][i];
+    for (int s = 0; s < U; s++) {
+        const uint32_t i = it + s * XV_TEAM;
+        // columns 2t, 2t + 1: token t / 2 of the pair, quad lanes 2 (t % 2) and the next
+        float2 f0[kSub], f1[kSub];  // this lane's scales, rows g and g + 8
+        if constexpr (FMT == LYTH_MX_NVFP4) {
+            const float2 a0 = mx_scales2<FMT>(q0[s]), a1 = mx_scales2<FMT>(q0[s] >> 16);
+            const float2 b0 = mx_scales2<FMT>(q1[s]), b1 = mx_scales2<FMT>(q1[s] >> 16);
+            f0[0] = make_float2(a0.x, a1.x);
+            f0[1] = make_float2(a0.y, a1.y);
+            f1[0] = make_float2(b0.x, b1.x);
+            f1[1] = make_float2(b0.y, b1.y);
+        } else if constexpr (FMT == LYTH_MX_FP4) {
+            f0[0] = mx_scales2<FMT>(q0[s] >> (16 * (t & 1)));
+            f1[0] = mx_scales2<FMT>(q1[s] >> (16 * (t & 1)));
+        } else {  // both columns in one block of 32
+            const uint32_t sh = 16 * (i & 1) + 8 * (t & 1);
+            f0[0].x = f0[0].y = mx_scales2<FMT>((q0[s] >> sh) & 0xFFu).x;
+            f1[0].x = f1[0].y = mx_scales2<FMT>((q1[s] >> sh) & 0xFFu).x;
         }
+#pragma unroll
+        for (int pr = 0; pr < PAIRS; pr++)
+#pragma unroll
+            for (int k = 0; k < kSub; k++) {
+                acc[pr][0] = __fmaf_rn(cc[s][pr][k][0], f0[k].x, acc[pr][0]);
+                acc[pr][1] = __fmaf_rn(cc[s][pr][k][2], f1[k].x, acc[pr][1]);
+                acc[pr][0] = __fmaf_rn(cc[s][pr][k][1], f0[k].y, acc[pr][0]);
+                acc[pr][1] = __fmaf_rn(cc[s][pr][k][3], f1[k].y, acc[pr][1]);
+            }
+    }
+}
+
+// Rows come in quads r, r + 32, r + 64, r + 96 of a scale tile, whose four scale words are contiguous.
+// Quad q's row in quarter j is 128 (q / 32) + q % 32 + 32 j. A block owns a contiguous range of quads
+// (the rows divide over the SMs to 4) in groups of four. PAIRS: token pairs (1, 2, 4).
+template <int FMT, int TY, int PAIRS>
+__global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_constant__ XvArgs p) {
+    using T = typename MxElem<TY>::type;
+    constexpr int kUnits = FMT == LYTH_MX_FP8 ? 2 : 4;    // 16-byte units of f16 x of a lane per step
+    constexpr int kU = PAIRS == 4 ? 1 : 2;                // steps a warp takes at once
+    constexpr uint32_t kStepX = 4 * kUnits * 16;          // bytes of x of a step and token
+    constexpr int kTokens = 2 * PAIRS;
+    extern __shared__ __align__(128) uint8_t sm[];        // ring, x, partial sums
+    __shared__ uint64_t bars[2 * 4 + 1];
+    __shared__ uint32_t s_max[XV_WARPS];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t xunits = p.chunk * XV_STEPS * 4 * kUnits;  // 16-byte units of x per token
+    uint4 *sx = reinterpret_cast<uint4 *>(sm + p.stages * Xv<FMT>::kStage);
+    float *s_part = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // [group][warp of its team][token][row]
+    auto full = [&](uint32_t s) { return smem_u32(bars + s); };
+    auto empty = [&](uint32_t s) { return smem_u32(bars + 4 + s); };
+    const uint32_t xbar = smem_u32(bars + 8);             // the consumers' meeting point
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; s++) {
+            mbar_init(full(s), 33 * XV_PRODUCERS);  // the producers' lanes (scales) and counts of bytes (rows)
+            mbar_init(empty(s), XV_TEAM);
+        }
+        mbar_init(xbar, XV_WARPS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < p.m * XV_ROWS; i += XV_THREADS) {
-        const uint32_t tok = i / XV_ROWS, r = i % XV_ROWS;
-        const uint64_t row = xv_row(tile, r);
-        if (row >= p.n) continue;
-        float v = 0.0f;
+
+    if (warp >= XV_WARPS && warp < XV_WARPS + XV_PRODUCERS) {  // ------------------------------------------------------------- producer
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        XvWalk w;
+        for (uint32_t b = 0; ok && xv_batch<kXvBatch<PAIRS>>(p, b, w); b++) {
+            const uint8_t *w_base = p.w + w.tile0 * 128 * p.row_bytes, *s_base = p.s + w.tile0 * p.words * 512;
+            for (uint32_t c0 = 0; ok && c0 < p.segs; c0 += p.chunk) {
+                const uint32_t c1 = min(c0 + p.chunk, p.segs);
+                for (uint32_t group = 0; ok && group < w.groups; group++) {
+                    // a warp per quad: lane j < 4 brings the row of quarter j, all lanes its scale words
+                    const uint32_t quad = w.lo + 4 * group + (warp - XV_WARPS), row = xv_row(quad, lane & 3);
+                    const bool has = quad < w.hi, has_row = lane < 4 && has && row <= w.last;
+                    const uint32_t rows = __popc(__ballot_sync(0xFFFFFFFFu, has_row));
+                    const uint8_t *src = w_base + (uint64_t)row * p.row_bytes;
+                    const uint8_t *ssrc = s_base + (uint64_t)(quad >> 5) * p.words * 512 + (quad & 31) * 16;
+                    for (uint32_t seg = c0; seg < c1; seg++) {
+                        if (!xv_wait(empty(stage), phase ^ 1)) { ok = false; break; }
+                        const uint32_t bytes = min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG);
+                        const uint32_t at = smem_u32(sm) + stage * Xv<FMT>::kStage;
+                        if (lane == 0) mbar_expect_tx(full(stage), rows * bytes);
+                        __syncwarp();
+                        if (has_row)
+                            bulk_load(at + ((warp - XV_WARPS) * 4 + lane) * XV_ROW, src + seg * XV_SEG, bytes, full(stage));
+                        const uint32_t w0 = seg * Xv<FMT>::kWords, nw = min(p.words - w0, (uint32_t)Xv<FMT>::kWords);
+                        if (has)
+                            for (uint32_t i = lane; i < nw; i += 32)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + XV_W_BYTES + i * 64 + (warp - XV_WARPS) * 16),
+                                             "l"(ssrc + (uint64_t)(w0 + i) * 512)
+                                             : "memory");
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(stage)) : "memory");
+                        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // Normally every copy has been consumed. After a timed-out wait, give the stages that may be in
+        // flight a bounded chance to land before the block leaves.
+        if (!ok)
+            for (uint32_t s = 0; s < p.stages; s++) {
+                xv_wait(full(stage), phase ^ 1);
+                if (++stage == p.stages) { stage = 0; phase ^= 1; }
+            }
+    } else if (warp < XV_WARPS) {  // ------------------------------------------------------ consumers
+        const uint32_t g = lane >> 2, t = lane & 3;
+        // x in shared memory: [token][step][unit][lane of the quad], tokens 64 bytes apart modulo 128, so
+        // that the eight lanes reading at once (two tokens, four quad lanes) reach all 32 banks. Lanes
+        // that hold no column keep zeros in xb: their loads are predicated off. Columns of tokens behind
+        // m are token m - 1 again and are not stored.
+        const bool mine = (g & 3) == t;
+        uint4 xb[4] = {};
+        uint32_t x_at[PAIRS];
 #pragma unroll
-        for (int k = 0; k < XV_WARPS; k++) v = __fadd_rn(v, s_part[k][tok][r]);
-        static_cast<T *>(p.y)[tok * p.ldy + row] = MxElem<TY>::round(__fmul_rn(p.alpha, __fmul_rn(v, unscale)));
+        for (int pr = 0; pr < PAIRS; pr++)
+            x_at[pr] = smem_u32(sx + min(2u * pr + (g >> 2), p.m - 1) * (xunits + 4) + t);
+        const T *x = static_cast<const T *>(p.x);
+        float scale = 1.0f;
+        // (rolled loops: code that runs once is fetched from memory as it runs)
+        if constexpr (TY == LYTH_NARROW_BF16) {
+            uint32_t top = 0;
+            for (uint32_t tok = 0; tok < p.m; tok++)
+#pragma unroll 1
+                for (uint32_t u = threadIdx.x; u < (p.cols + 7) / 8; u += 32 * XV_WARPS)
+                    top = max(top, xv_top(xv_load8<TY>(x + tok * p.ldx, 8 * u, p.cols, p.vec)));
+            top = __reduce_max_sync(0xFFFFFFFFu, top);
+            if (lane == 0) s_max[warp] = top;
+            xv_sync_consumers();
+            top = __reduce_max_sync(0xFFFFFFFFu, lane < XV_WARPS ? s_max[lane] : 0u);
+            // 2^(14 - e), e the largest exponent; it and its inverse kept within normal f32 numbers
+            const int sh = min(14 - ((int)top - 127), 126);
+            scale = __uint_as_float((uint32_t)(sh + 127) << 23);
+        }
+        const float unscale = __uint_as_float((254u << 23) - __float_as_uint(scale));
+        uint32_t stage = 0, phase = 0;
+        bool ok = true, staged = false;
+        uint32_t xphase = 0;
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(xbar);
+            const bool met = xv_wait(xbar, xphase);
+            xphase ^= 1;
+            return met;
+        };
+        XvWalk w;
+        for (uint32_t b = 0; ok && xv_batch<kXvBatch<PAIRS>>(p, b, w); b++) {
+            for (uint32_t c0 = 0; ok && c0 < p.segs; c0 += p.chunk) {
+                if (!staged || p.chunk < p.segs) {
+                    // (a bounded meeting: a warp that gave up a wait has left)
+                    if (staged && !(ok = meet())) break;
+                    const uint32_t first = c0 * XV_STEPS * 4 * kUnits;
+                    for (uint32_t tok = 0; tok < p.m; tok++)
+#pragma unroll 1
+                        for (uint32_t u = threadIdx.x; u < xunits; u += 32 * XV_WARPS) {
+                            const uint32_t at = u / (4 * kUnits) * (4 * kUnits) + u % kUnits * 4 + u / kUnits % 4;
+                            sx[tok * (xunits + 4) + at] =
+                                xv_f16<TY>(xv_load8<TY>(x + tok * p.ldx, 8 * (first + u), p.cols, p.vec), scale);
+                        }
+                    if (!(ok = meet())) break;
+                    staged = true;
+                }
+                const uint32_t c1 = min(c0 + p.chunk, p.segs);
+                for (uint32_t group = 0; ok && group < w.groups; group++) {
+                    if ((group & 1) != warp / XV_TEAM) {  // the other team's
+                        for (uint32_t seg = c0; seg < c1; seg++)
+                            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                        continue;
+                    }
+                    float acc[PAIRS][2] = {};
+                    for (uint32_t seg = c0; seg < c1; seg++) {
+                        if (!xv_wait(full(stage), phase)) { ok = false; break; }
+                        const uint8_t *at = sm + stage * Xv<FMT>::kStage;
+                        const uint32_t steps = (min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG) + 63) / 64;
+                        const uint32_t words = p.words - seg * Xv<FMT>::kWords, x_base = (seg - c0) * XV_STEPS * kStepX;
+                        uint32_t it = warp % XV_TEAM;
+                        for (; it + (kU - 1) * XV_TEAM < steps; it += kU * XV_TEAM)
+                            xv_steps<FMT, PAIRS, kU>(at, it, x_base + it * kStepX, g, t, mine, x_at, words, xb, acc);
+                        if constexpr (kU > 1)
+                            for (; it < steps; it += XV_TEAM)
+                                xv_steps<FMT, PAIRS, 1>(at, it, x_base + it * kStepX, g, t, mine, x_at, words, xb, acc);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(empty(stage));
+                        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                    }
+                    if (!ok) break;
+                    // this warp's part of the group, of its own from chunk to chunk
+                    float *part = s_part + (group * XV_TEAM + warp % XV_TEAM) * (kTokens * 16);
+#pragma unroll
+                    for (int pr = 0; pr < PAIRS; pr++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float v = __fadd_rn(acc[pr][i], __shfl_xor_sync(0xFFFFFFFFu, acc[pr][i], 1));
+                            float *to = part + (2 * pr + (t >> 1)) * 16 + g + 8 * i;
+                            if ((t & 1) == 0) *to = c0 ? __fadd_rn(*to, v) : v;
+                        }
+                }
+            }
+            if (!ok || !(ok = meet())) break;
+#pragma unroll 1
+            for (uint32_t i = threadIdx.x; i < w.groups * p.m * 16; i += 32 * XV_WARPS) {
+                const uint32_t group = i / 16 % w.groups, tok = i / 16 / w.groups, r = i & 15;
+                const uint32_t quad = w.lo + 4 * group + (r >> 2), row = xv_row(quad, r & 3);
+                const float *part = s_part + (group * XV_TEAM * kTokens + tok) * 16 + r;
+                float v = 0.0f;
+#pragma unroll
+                for (int k = 0; k < XV_TEAM; k++) v = __fadd_rn(v, part[k * kTokens * 16]);
+                if (quad < w.hi && row <= w.last)
+                    static_cast<T *>(p.y)[tok * p.ldy + w.tile0 * 128 + row] =
+                        MxElem<TY>::round(__fmul_rn(p.alpha, __fmul_rn(v, unscale)));
+            }
+            if (w.hi - w.lo == 4 * kXvBatch<PAIRS> && !(ok = meet())) break;  // before the next batch's sums
+        }
     }
 }
 
 template <int FMT, int TY, int PAIRS>
 static int xv_launch(XvArgs p, cudaStream_t s) {
-    // x of one step takes 2 PAIRS x 4 lanes x kUnits x 16 bytes; 64 KiB of it at once
-    const uint32_t step_bytes = 2 * PAIRS * (FMT == LYTH_MX_FP8 ? 8 : 16) * 16;
-    const uint32_t most = 64 * 1024 / step_bytes;
-    p.chunk = p.iters < most ? p.iters : most;
-    const size_t smem = (size_t)p.chunk * step_bytes;
-    if (smem > 40 * 1024) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(mx_gemv_kernel<FMT, TY, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // Shared memory: the partial sums, a ring of 3 or 4 stages, and as many segments of x as are left
+    // room for (at least one: 8 tokens x 2048 E2M1 bytes are 64 KiB).
+    const size_t seg_x = (size_t)p.m * XV_STEPS * (FMT == LYTH_MX_FP8 ? 8 : 16) * 16;
+    const size_t fixed = (size_t)kXvBatch<PAIRS> * XV_TEAM * 2 * PAIRS * 16 * sizeof(float) + p.m * 64;
+    const size_t room = 226 * 1024 - fixed;
+    p.stages = 4;
+    if (4 * (size_t)Xv<FMT>::kStage + p.segs * seg_x > room) p.stages = 3;
+    const size_t most = (room - p.stages * (size_t)Xv<FMT>::kStage) / seg_x;
+    p.chunk = p.segs < most ? p.segs : (uint32_t)most;
+    const size_t smem = p.stages * (size_t)Xv<FMT>::kStage + p.chunk * seg_x + fixed;
+    static size_t set[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return status_of(e);
+    if (dev < 0 || dev >= 64 || set[dev] == 0) {
+        e = cudaFuncSetAttribute(mx_gemv_kernel<FMT, TY, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
         if (e != cudaSuccess) return status_of(e);
+        if (dev >= 0 && dev < 64) set[dev] = 1;
     }
-    const unsigned grid = (unsigned)((p.n + 127) / 128 * 8);
+    const uint32_t quads = p.n / 128 * 32 + (p.n % 128 < 32 ? p.n % 128 : 32u);
+    const uint32_t sms = (uint32_t)device_sms(), grid = quads < sms ? quads : sms;
+    p.quads_each = quads / grid;
+    p.quads_more = quads % grid;
     mx_gemv_kernel<FMT, TY, PAIRS><<<grid, XV_THREADS, smem, s>>>(p);
     return last_launch_status();
 }
@@ -221,6 +456,16 @@ static int xv_pairs(const XvArgs &p, cudaStream_t s) {
     return xv_launch<FMT, TY, 4>(p, s);
 }
 
+int xv_take_device_error() {
+    int v = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_xv_error, sizeof(int));
+    if (e != cudaSuccess) return status_of(e);
+    if (!v) return LYTH_OK;
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_xv_error, &zero, sizeof(int));
+    return LYTH_E_TIMEOUT;
+}
+
 }  // namespace lyth
 
 using namespace lyth;
@@ -230,7 +475,7 @@ extern "C" int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32
                                  cudaStream_t s) {
     if (!mx_known(fmt) || (ty != LYTH_NARROW_F16 && ty != LYTH_NARROW_BF16) || m > LYTH_GEMV_MX_MAX_M)
         return LYTH_E_UNSUPPORTED;
-    if (cols == 0 || cols > (1u << 30) || n > (1u << 31) || ldx < cols || ldy < n) return LYTH_E_INVALID;
+    if (cols == 0 || cols > (1u << 24) || n > (1u << 31) || ldx < cols || ldy < n) return LYTH_E_INVALID;
     if (m == 0 || n == 0) return LYTH_OK;
     if (!x || !w || !w_scales || !y) return LYTH_E_INVALID;
     if (!aligned16(w) || !aligned16(w_scales)) return LYTH_E_UNSUPPORTED;
@@ -247,7 +492,7 @@ extern "C" int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32
     p.cols = cols;
     p.row_bytes = (uint32_t)mx_code_bytes(fmt, k);
     p.words = (uint32_t)(k / (4 * mx_block(fmt)));
-    p.iters = (p.row_bytes + 63) / 64;
+    p.segs = (p.row_bytes + XV_SEG - 1) / XV_SEG;
     p.alpha = alpha;
     p.vec = aligned16(x) && ldx * 2 % 16 == 0;
     const bool bf = ty == LYTH_NARROW_BF16;
