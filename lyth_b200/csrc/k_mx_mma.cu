@@ -15,6 +15,7 @@
 // Ragged edges: rows behind m or n arrive as zeros (tensor-map fill) or carry any scale, and are not
 // stored; k is whole scale words, so the last step's MMAs are only fewer. Every wait is bounded.
 #include <cuda.h>
+#include <stdlib.h>
 
 #include "mbar.cuh"
 #include "mx.cuh"
@@ -103,21 +104,31 @@ struct XmArgs {
     uint32_t row_bytes;      // bytes of a row of codes
     uint32_t words;          // scale tiles along k
     float alpha;
-    bool vec;                // rows of C start on 16 bytes
+    bool vec;                // rows of C start on 32 bytes
 };
 
-// 32 accumulators of one row to C, columns col .. col + 31.
+// 32 accumulators of one row to C, columns col .. col + 31: in 256-bit stores, a whole sector each,
+// where rows start on 32 bytes.
 template <int TY>
 LYTH_D void xm_store32(typename MxElem<TY>::type *crow, uint64_t col, uint64_t n, bool vec, float alpha,
                        const uint32_t (&r)[32]) {
     if (col >= n) return;
     const uint32_t left = n - col < 32 ? (uint32_t)(n - col) : 32u;
 #pragma unroll
-    for (int v = 0; v < 4; v++) {
-        float f[8];
+    for (int v = 0; v < 2; v++) {
+        float f[16];
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = __fmul_rn(alpha, __uint_as_float(r[8 * v + i]));
-        mx_store8<TY>(crow + col, 8 * v, left, vec, f);
+        for (int i = 0; i < 16; i++) f[i] = __fmul_rn(alpha, __uint_as_float(r[16 * v + i]));
+        if (vec && 16u * v + 16 <= left) {
+            uint32_t w[kMxWords<TY>];
+            mx_narrow<TY>(f, w);
+#pragma unroll
+            for (int i = 0; i < kMxWords<TY>; i += 8) mx_st32(reinterpret_cast<uint32_t *>(crow + col + 16 * v) + i, w + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (16u * v + i < left) crow[col + 16 * v + i] = MxElem<TY>::round(f[i]);
+        }
     }
 }
 
@@ -253,6 +264,258 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// The 2-SM form: a CTA pair computes a 256 x 192 tile with tcgen05.mma.cta_group::2. Each CTA stages
+// its 128 rows of A and 96 of the tile's 192 rows of B, so a 128-byte step moves 28 KiB into an SM for
+// the work that takes the 128 x 128 form 42 KiB: at 4 bits that form is bound by this traffic, not by
+// the tensor cores. 192 columns leave room in tensor memory for two accumulators (2 x 192) beside two
+// sets of scales (2 x 48): the epilogue runs beside the next tile, which 256 columns would not allow.
+//
+//   both CTAs, warp 0    producer: its halves of A and B as boxes that complete on the leader's `full`
+//                        barrier; its 128 rows' A scales and the B scales of all 192 columns (the pair's
+//                        MMA reads them in each CTA's tensor memory) on its own `sfull`. No multicast.
+//   both CTAs, warps 6-9 scales: from shared to tensor memory, each warp its 32-lane quadrant (the four
+//                        quadrants hold the same scales), then an arrival on the leader's `sready`.
+//                        tcgen05.cp does this without warps, but in the MMAs' queue: a copy of one tile
+//                        took 60 cycles of it, twelve of them (NVFP4) twice the time of the step's MMAs.
+//   leader, warp 1       issues the MMAs; one commit frees the stage, and the set of scales in tensor
+//                        memory, in both CTAs.
+//   both CTAs, warps 2-5 epilogue of this CTA's 128 rows.
+// B scale tiles are 128 rows and the tile's 192 start on a multiple of 64: two tiles cover them, and
+// an odd start reads from two tensor-memory columns (64 rows) on.
+constexpr int X2_BN = 192, X2_HALF = X2_BN / 2;
+constexpr int X2_B_BYTES = X2_HALF * 128;
+constexpr uint32_t X2_SF_COL = 2 * X2_BN;
+constexpr int X2_THREADS = 320;
+
+template <int FMT>
+struct X2 {
+    static constexpr int kTiles = Xm<FMT>::kTiles;
+    static constexpr int kStageBytes = XM_OP_BYTES + X2_B_BYTES + 3 * kTiles * 512;
+    static constexpr int kSetCols = 12 * kTiles;                     // a step's scales in tensor memory
+    static constexpr int kSets = 128 / kSetCols < 4 ? 128 / kSetCols : 4;
+    static constexpr int kStages = 225 * 1024 / kStageBytes;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + 256;
+};
+
+LYTH_D void x2_tma2(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+LYTH_D void x2_tma3_own(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+LYTH_D void x2_st4(uint32_t taddr, uint4 v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+template <int FMT>
+LYTH_D void x2_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+#define LYTH_X2_MMA(KIND)                                                                                  \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                         \
+                 "tcgen05.mma.cta_group::2." KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),       \
+                 "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)                                \
+                 : "memory")
+    if constexpr (FMT == LYTH_MX_FP8) LYTH_X2_MMA("kind::mxf8f6f4.block_scale.scale_vec::1X");
+    else if constexpr (FMT == LYTH_MX_FP4) LYTH_X2_MMA("kind::mxf4.block_scale.scale_vec::2X");
+    else LYTH_X2_MMA("kind::mxf4nvf4.block_scale.scale_vec::4X");
+#undef LYTH_X2_MMA
+}
+LYTH_D void x2_commit(uint32_t bar) {  // on this barrier in both CTAs
+    const uint16_t mask = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(mask)
+        : "memory");
+}
+
+template <int FMT, int TY>
+__global__ void __launch_bounds__(X2_THREADS, 1)
+    mx_mma2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                   typename MxElem<TY>::type *C, XmArgs p) {
+    constexpr int T = X2<FMT>::kTiles, S = X2<FMT>::kStages, kSets = X2<FMT>::kSets;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * X2_B_BYTES, *sSB = sSA + S * T * 512;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + S * 2 * T * 512);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 4 + 4);
+    auto full = [&](int s) { return smem_u32(bars + s); };
+    auto empty = [&](int s) { return smem_u32(bars + S + s); };
+    auto sfull = [&](int s) { return smem_u32(bars + 2 * S + s); };
+    auto tfull = [&](int b) { return smem_u32(bars + 3 * S + b); };
+    auto tempty = [&](int b) { return smem_u32(bars + 3 * S + 2 + b); };
+    auto sready = [&](int b) { return smem_u32(bars + 3 * S + 4 + b); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t crank = cluster_ctarank();
+    uint32_t pair, npairs;
+    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(pair));
+    asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(npairs));
+    const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + X2_BN - 1) / X2_BN, ntiles = tiles_m * tiles_n;
+    const uint32_t steps = (p.row_bytes + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(full(s), 2);  // the two producers' arrivals (the leader's barrier is the one used)
+            mbar_init(empty(s), 1);
+            mbar_init(sfull(s), 1);
+        }
+        for (int b = 0; b < kSets; b++) mbar_init(sready(b), 8);  // four scale warps in each CTA (the leader's)
+        for (int b = 0; b < 2; b++) {
+            mbar_init(tfull(b), 1);
+            mbar_init(tempty(b), 8);  // four epilogue warps in each CTA (the leader's is the one used)
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(XM_TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    xm_fence_before();
+    cluster_sync_all();
+    xm_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
+                const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
+                const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * X2_BN);
+                for (uint32_t kb = 0; kb < steps; kb++) {
+                    if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
+                    const uint32_t lf = mapa_shared(full(stage), 0);
+                    mbar_expect_tx(sfull(stage), 3 * T * 512);
+                    x2_tma3_own(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
+                    x2_tma3_own(smem_u32(sSB + stage * 2 * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
+                    mbar_expect_tx_cluster(lf, XM_OP_BYTES + X2_B_BYTES);
+                    x2_tma2(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), m0, lf);
+                    x2_tma2(smem_u32(sB + stage * X2_B_BYTES), &tmB, (int)(kb * 128), n0 + X2_HALF * (int)crank, lf);
+                    if (++stage == S) { stage = 0; phase ^= 1; }
+                }
+            }
+            // Tail: every stage released by the MMA's commit, so no arrival is still on its way to
+            // this CTA's barriers when it leaves.
+            if (ok)
+                for (int s = 0; s < S; s++) {
+                    if (!xm_wait(empty(stage), phase ^ 1)) break;
+                    if (++stage == S) { stage = 0; phase ^= 1; }
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && crank == 0) {
+            uint32_t stage = 0, phase = 0, local = 0, set = 0, sphase = 0;
+            bool ok = true;
+            for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
+                const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
+                if (!xm_wait(tempty(ab), aphase ^ 1)) { ok = false; break; }
+                xm_fence_after();
+                const uint32_t d = tmem_base + ab * X2_BN;
+                const uint32_t shift = ((uint32_t)(tile / tiles_m) & 1) * 2;  // 192 tn is 64 mod 128
+                for (uint32_t kb = 0; kb < steps; kb++) {
+                    if (!xm_wait(full(stage), phase) || !xm_wait(sready(set), sphase)) { ok = false; break; }
+                    xm_fence_after();
+                    const uint32_t left = p.row_bytes - kb * 128;
+                    const int mmas = left < 128 ? (int)(left / 32) : 4;
+                    const uint32_t sfa = tmem_base + X2_SF_COL + set * X2<FMT>::kSetCols, sfb = sfa + 4 * T;
+                    const uint32_t a = smem_u32(sA + stage * XM_OP_BYTES), b = smem_u32(sB + stage * X2_B_BYTES);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (j < mmas)
+                            x2_mma<FMT>(d, xm_desc_op(a + 32 * j), xm_desc_op(b + 32 * j), xm_idesc<FMT>(X2_BN, 256, j),
+                                        sfa + 4 * (j * T / 4), sfb + 8 * (j * T / 4) + shift, (kb | (uint32_t)j) != 0);
+                    }
+                    x2_commit(empty(stage));
+                    if (++stage == S) { stage = 0; phase ^= 1; }
+                    if (++set == kSets) { set = 0; sphase ^= 1; }
+                }
+                if (ok) x2_commit(tfull(ab));
+            }
+            // After a timed-out wait, give the stages the producers may have in flight a bounded
+            // chance to land (both CTAs' copies complete on these barriers) before the pair leaves.
+            if (!ok) {
+                for (int s = 0; s < S; s++) {
+                    xm_wait(full(stage), phase);
+                    if (++stage == S) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+    } else if (warp >= 6) {
+        const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may write
+        uint32_t stage = 0, phase = 0, set = 0, lead[kSets];
+        for (int b = 0; b < kSets; b++) lead[b] = mapa_shared(sready(b), 0);
+        uint32_t step = 0, old = 0, old_phase = 0;  // steps so far; the stage and phase of the one kSets back
+        bool ok = true;
+        for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
+            for (uint32_t kb = 0; kb < steps; kb++) {
+                // the set is free once the MMAs of the step kSets back, whose commit frees its stage, are done
+                if (step >= (uint32_t)kSets) {
+                    if (!xm_wait(empty(old), old_phase)) { ok = false; break; }
+                    if (++old == S) { old = 0; old_phase ^= 1; }
+                } else {
+                    step++;
+                }
+                if (!xm_wait(sfull(stage), phase)) { ok = false; break; }
+                xm_fence_after();
+                const uint32_t at = tmem_base + ((quad * 32) << 16) + X2_SF_COL + set * X2<FMT>::kSetCols;
+                // a tile is 16 bytes a lane: its words of four columns
+                const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * 2 * T * 512 + lane * 16;
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    x2_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(a + t * 512));
+                    x2_st4(at + 4 * T + 8 * t, *reinterpret_cast<const uint4 *>(b + t * 512));
+                    x2_st4(at + 4 * T + 8 * t + 4, *reinterpret_cast<const uint4 *>(b + (T + t) * 512));
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                xm_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead[set]);
+                if (++stage == S) { stage = 0; phase ^= 1; }
+                if (++set == kSets) set = 0;
+            }
+        }
+    } else {
+        const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may read
+        const uint32_t lead_tempty[2] = {mapa_shared(tempty(0), 0), mapa_shared(tempty(1), 0)};
+        uint32_t local = 0;
+        for (uint64_t tile = pair; tile < ntiles; tile += npairs, local++) {
+            const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
+            if (!xm_wait(tfull(ab), aphase)) break;
+            xm_fence_after();
+            const uint64_t row = tile % tiles_m * 256 + 128 * crank + quad * 32 + lane, n0 = tile / tiles_m * X2_BN;
+#pragma unroll 1
+            for (int c = 0; c < X2_BN / 32; c++) {
+                uint32_t r[32];
+                xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
+                if (row < p.m) xm_store32<TY>(C + row * p.ldc, n0 + c * 32, p.n, p.vec, p.alpha, r);
+            }
+            xm_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(lead_tempty[ab]);
+        }
+    }
+    __syncwarp();
+    xm_fence_before();
+    cluster_sync_all();
+    if (warp == 1) {
+        xm_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(XM_TMEM_COLS)
+                     : "memory");
+    }
+}
+
 // Codes as a 2-D byte tensor: a 128-byte (the swizzle span) x box_rows box, zeros outside.
 static bool xm_map(CUtensorMap *map, const void *base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows) {
     PFN_encode_tiled enc = tensor_map_encoder();
@@ -264,6 +527,63 @@ static bool xm_map(CUtensorMap *map, const void *base, uint64_t row_bytes, uint6
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Scale tiles as a 3-D tensor of words: 128 (512 bytes) x tiles along k x tiles of 128 rows.
+static bool xm_map_sf(CUtensorMap *map, const void *base, uint64_t words, uint64_t rows, uint32_t box_words,
+                      uint32_t box_tiles) {
+    PFN_encode_tiled enc = tensor_map_encoder();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {128, words, (rows + 127) / 128};
+    cuuint64_t strides[2] = {512, words * 512};
+    cuuint32_t box[3] = {128, box_words, box_tiles};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, int TY>
+static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &p, cudaStream_t s) {
+    constexpr int T = X2<FMT>::kTiles;
+    CUtensorMap ta, tb, tsa, tsb;
+    if (!xm_map(&ta, a, p.row_bytes, p.m, 128) || !xm_map(&tb, b, p.row_bytes, p.n, X2_HALF) ||
+        !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, 2))
+        return LYTH_E_UNSUPPORTED;
+    static int fit_of[64] = {0};  // pairs resident at once, asked once per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return status_of(e);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(X2_THREADS);
+    cfg.dynamicSmemBytes = X2<FMT>::kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int pairs = device_sms() / 2;
+    if (dev < 0 || dev >= 64 || fit_of[dev] == 0) {
+        e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)X2<FMT>::kSmem);
+        if (e != cudaSuccess) return status_of(e);
+        cfg.gridDim = dim3(2u * (unsigned)pairs);
+        int fit = 0;
+        if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
+        cudaGetLastError();
+        if (fit < pairs) pairs = fit;
+        if (dev >= 0 && dev < 64) fit_of[dev] = pairs;
+    } else {
+        pairs = fit_of[dev];
+    }
+    const uint64_t tiles = (p.m + 255) / 256 * ((p.n + X2_BN - 1) / X2_BN);
+    if ((uint64_t)pairs > tiles) pairs = (int)tiles;
+    cfg.gridDim = dim3(2u * (unsigned)pairs);
+    e = cudaLaunchKernelEx(&cfg, mx_mma2_kernel<FMT, TY>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p);
+    if (e != cudaSuccess) return status_of(e);
+    return last_launch_status();
 }
 
 template <int FMT, int TY>
@@ -302,7 +622,7 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
                                    const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, float alpha,
                                    void *c, uint64_t ldc, cudaStream_t s) {
     if (!mx_known(fmt) || !mx_ty_known(ty)) return LYTH_E_UNSUPPORTED;
-    if (cols == 0 || cols > (1u << 30) || m > (1u << 31) || n > (1u << 31) || ldc < n) return LYTH_E_INVALID;
+    if (cols == 0 || cols > (1u << 30) || m > 0x7FFFFE00u || n > 0x7FFFFE00u || ldc < n) return LYTH_E_INVALID;
     if (m == 0 || n == 0) return LYTH_OK;
     if (!a || !a_scales || !b || !b_scales || !c) return LYTH_E_INVALID;
     if (!aligned16(a) || !aligned16(a_scales) || !aligned16(b) || !aligned16(b_scales)) return LYTH_E_UNSUPPORTED;
@@ -316,7 +636,10 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     p.row_bytes = (uint32_t)mx_code_bytes(fmt, k);
     p.words = (uint32_t)(k / (4 * mx_block(fmt)));
     p.alpha = alpha;
-    p.vec = aligned16(c) && ldc * mx_ty_bytes(ty) % 16 == 0;
+    p.vec = aligned32(c) && ldc * mx_ty_bytes(ty) % 32 == 0;
+    if (getenv("X2") ? atoi(getenv("X2")) : m > 128) {
+        LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY>(a, b, c, p, s)));
+    }
     CUtensorMap ta, tb;
     if (!xm_map(&ta, a, p.row_bytes, m, XM_BM) || !xm_map(&tb, b, p.row_bytes, n, XM_BN)) return LYTH_E_UNSUPPORTED;
     LYTH_MX_DISPATCH(fmt, ty, return (xm_launch<FMT, TY>(ta, tb, c, p, s)));

@@ -98,23 +98,6 @@ LYTH_D void mx_load8(const typename MxElem<TY>::type *row, uint32_t col, uint32_
         for (int i = 0; i < 8; i++) v[i] = col + i < cols ? MxElem<TY>::load(row + col + i) : 0.0f;
     }
 }
-template <int TY>
-LYTH_D void mx_store8(typename MxElem<TY>::type *row, uint32_t col, uint32_t cols, bool vec, const float (&v)[8]) {
-    if (vec && col + 8 <= cols) {
-        if constexpr (TY == 0) {
-            *reinterpret_cast<float4 *>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4 *>(row + col + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(row + col) = make_uint4(mx_pack2<TY>(v[0], v[1]), mx_pack2<TY>(v[2], v[3]),
-                                                               mx_pack2<TY>(v[4], v[5]), mx_pack2<TY>(v[6], v[7]));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (col + i < cols) row[col + i] = MxElem<TY>::round(v[i]);
-    }
-}
-
 // ---- rows of the unquantised side, 16 values ("a chunk") at a time.
 // A chunk is 8 words of a 16-bit type, 16 of f32. VEC: every row starts on 32 bytes and is whole
 // chunks, which move in 256-bit accesses (two 128-bit stores 32 bytes apart per lane write every
