@@ -26,8 +26,9 @@ __device__ int g_mx_error = 0;
 
 constexpr int XM_BM = 128, XM_BN = 128, XM_STAGES = 6, XM_THREADS = 192;
 constexpr int XM_OP_BYTES = 128 * 128;         // one operand's box: 128 rows x 128 bytes
-constexpr int XM_TMEM_COLS = 512;              // two 128-column accumulators, then the scales
-constexpr uint32_t XM_SF_COL = 2 * XM_BN;
+constexpr int XM_TMEM_COLS = 512;              // the pair form: two accumulators, then the scales
+constexpr int X1_TMEM_COLS = 256;              // the single-SM form: an accumulator, then the scales
+constexpr uint32_t X1_PITCH = XM_BN + 4;
 
 // Scale tiles (4 blocks along k) in one 128-byte step.
 template <int FMT>
@@ -49,17 +50,24 @@ LYTH_D uint32_t xm_idesc(int n, int m, int j) {
            ((FMT == LYTH_MX_NVFP4 ? 0u : 1u) << 23) | ((uint32_t)(m >> 7) << 27) | (id << 29);
 }
 
-LYTH_D bool xm_wait(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, &g_mx_error); }
+// Every role is a whole warp in step: its lanes wait together, take one decision by vote, and one elected
+// lane issues. The operands of TMA and MMA instructions then stay in uniform registers; a loop of a
+// single lane (`if (lane == 0)`) had the compiler gather them for each instruction, 880 cycles for the
+// four MMAs and two waits of a step and 550 for its four copies, which bound the kernels.
+LYTH_D bool xm_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, &g_mx_error));
+}
+LYTH_D bool xm_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+LYTH_D uint32_t xm_uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
 
-// Shared-memory descriptors: K-major rows of 128 bytes with the 128-byte swizzle (8-row groups 1024
-// bytes apart), and the unswizzled 32 x 16-byte scale tile (8-row groups 128 bytes apart).
+// Shared-memory descriptor: K-major rows of 128 bytes with the 128-byte swizzle (8-row groups 1024
+// bytes apart).
 LYTH_D uint64_t xm_desc_op(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
-}
-LYTH_D uint64_t xm_desc_sf(uint32_t addr) { return (uint64_t)((addr >> 4) & 0x3FFFu) | 8ull << 32 | 1ull << 46; }
-
-LYTH_D void xm_copy_sf(uint32_t tmem, uint32_t smem) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(xm_desc_sf(smem)) : "memory");
 }
 
 template <int FMT>
@@ -132,134 +140,197 @@ LYTH_D void xm_store32(typename MxElem<TY>::type *crow, uint64_t col, uint64_t n
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// The single-SM form, for products of at most one 128 x 128 tile per SM: a cluster of KS CTAs (1, 2, 4
+// or 8) takes a tile, each a contiguous share of k, so that few tiles still fill the machine; their
+// accumulators meet in shared memory and every CTA adds up a share of the columns over the cluster, in
+// rank order. One token batch of 32 through 14336 x 4096 is 112 tiles; through 4096 x 14336, 32 tiles
+// of four shares.
+//   warp 0     producer: boxes of A (only the rows that exist), B and both operands' scales.
+//   warp 1     issues the MMAs.
+//   warps 2-5  scales from shared to tensor memory as below, then the epilogue.
+constexpr int X1_SETS = 4;
+
+LYTH_D void x1_st4(uint32_t taddr, uint4 v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+LYTH_D void xm_tma3(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
 template <int FMT, int TY>
 __global__ void __launch_bounds__(XM_THREADS, 1)
-    mx_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                  typename MxElem<TY>::type *C, XmArgs p) {
-    constexpr int T = Xm<FMT>::kTiles;
+    mx_mma1_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                   typename MxElem<TY>::type *C, XmArgs p, uint32_t ks, uint32_t a_rows) {
+    constexpr int T = Xm<FMT>::kTiles, S = XM_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = sA + XM_STAGES * XM_OP_BYTES, *sSA = sB + XM_STAGES * XM_OP_BYTES;
-    uint8_t *sSB = sSA + XM_STAGES * T * 512;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + XM_STAGES * T * 512);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * XM_STAGES + 4);
+    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * XM_OP_BYTES, *sSB = sSA + S * T * 512;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + S * T * 512);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + X1_SETS + 1);
     auto full = [&](int s) { return smem_u32(bars + s); };
-    auto empty = [&](int s) { return smem_u32(bars + XM_STAGES + s); };
-    auto tfull = [&](int b) { return smem_u32(bars + 2 * XM_STAGES + b); };
-    auto tempty = [&](int b) { return smem_u32(bars + 2 * XM_STAGES + 2 + b); };
+    auto empty = [&](int s) { return smem_u32(bars + S + s); };
+    auto sready = [&](int b) { return smem_u32(bars + 2 * S + b); };
+    const uint32_t done = smem_u32(bars + 2 * S + X1_SETS);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t tiles_m = (p.m + XM_BM - 1) / XM_BM, tiles_n = (p.n + XM_BN - 1) / XM_BN, ntiles = tiles_m * tiles_n;
-    const uint32_t steps = (p.row_bytes + 127) / 128;
+    const int warp = (int)xm_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x % ks, tile = blockIdx.x / ks;
+    const uint32_t tiles_m = (uint32_t)((p.m + XM_BM - 1) / XM_BM), tm = tile % tiles_m, tn = tile / tiles_m;
+    const uint32_t all = (p.row_bytes + 127) / 128, k0 = all * rank / ks, k1 = all * (rank + 1) / ks;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < XM_STAGES; s++) {
+        for (int s = 0; s < S; s++) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        for (int b = 0; b < 2; b++) {
-            mbar_init(tfull(b), 1);
-            mbar_init(tempty(b), 4);
-        }
+        for (int b = 0; b < X1_SETS; b++) mbar_init(sready(b), 4);
+        mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(XM_TMEM_COLS)
+                     "r"(X1_TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     xm_fence_before();
     __syncthreads();
     xm_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = xm_uniform(*tmem_slot);
+    bool ok = true;
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            bool ok = true;
-            for (uint64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x) {
-                const uint64_t tm = tile % tiles_m, tn = tile / tiles_m;
-                const uint8_t *sa = p.sa + tm * p.words * 512, *sb = p.sb + tn * p.words * 512;
-                for (uint32_t kb = 0; kb < steps; kb++) {
-                    if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
-                    const uint32_t w0 = kb * T, nw = p.words - w0 < T ? p.words - w0 : T;
-                    mbar_expect_tx(full(stage), 2 * XM_OP_BYTES + 2 * nw * 512);
-                    xm_tma(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), (int)(tm * XM_BM), full(stage));
-                    xm_tma(smem_u32(sB + stage * XM_OP_BYTES), &tmB, (int)(kb * 128), (int)(tn * XM_BN), full(stage));
-                    bulk_load(smem_u32(sSA + stage * T * 512), sa + (uint64_t)w0 * 512, nw * 512, full(stage));
-                    bulk_load(smem_u32(sSB + stage * T * 512), sb + (uint64_t)w0 * 512, nw * 512, full(stage));
-                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
-                }
+        uint32_t stage = 0, phase = 0;
+        for (uint32_t kb = k0; kb < k1; kb++) {
+            if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
+            if (xm_elect()) {
+                mbar_expect_tx(full(stage), a_rows * 128 + XM_OP_BYTES + 2 * T * 512);
+                xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), (int)tm, full(stage));
+                xm_tma3(smem_u32(sSB + stage * T * 512), &tmSB, 0, (int)(kb * T), (int)tn, full(stage));
+                xm_tma(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), (int)(tm * XM_BM), full(stage));
+                xm_tma(smem_u32(sB + stage * XM_OP_BYTES), &tmB, (int)(kb * 128), (int)(tn * XM_BN), full(stage));
             }
-            // After a timed-out wait, give the stages this thread may have in flight a bounded
-            // chance to land before the block leaves.
-            if (!ok) {
-                for (int s = 0; s < XM_STAGES; s++) {
-                    xm_wait(full(stage), phase);
-                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
-                }
+            __syncwarp();
+            if (++stage == S) { stage = 0; phase ^= 1; }
+        }
+        // After a timed-out wait, give the stages that may be in flight a bounded chance to land before
+        // the block leaves.
+        if (!ok) {
+            for (int s = 0; s < S; s++) {
+                xm_wait(full(stage), phase);
+                if (++stage == S) { stage = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0, local = 0;
-            bool ok = true;
-            for (uint64_t tile = blockIdx.x; tile < ntiles && ok; tile += gridDim.x, local++) {
-                const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
-                if (!xm_wait(tempty(ab), aphase ^ 1)) break;
-                xm_fence_after();
-                const uint32_t d = tmem_base + ab * XM_BN;
-                for (uint32_t kb = 0; kb < steps; kb++) {
-                    if (!xm_wait(full(stage), phase)) { ok = false; break; }
-                    xm_fence_after();
-                    const uint32_t left = p.row_bytes - kb * 128;
-                    const int mmas = left < 128 ? (int)(left / 32) : 4;
-                    const uint32_t sfa = tmem_base + XM_SF_COL + (kb & 1) * 32, sfb = sfa + 16;
-                    const uint32_t a = smem_u32(sA + stage * XM_OP_BYTES), b = smem_u32(sB + stage * XM_OP_BYTES);
+        uint32_t stage = 0, phase = 0, set = 0, sphase = 0;
+        for (uint32_t kb = k0; kb < k1; kb++) {
+            if (!xm_wait(full(stage), phase) || !xm_wait(sready(set), sphase)) { ok = false; break; }
+            xm_fence_after();
+            const uint32_t left = p.row_bytes - kb * 128;
+            const int mmas = left < 128 ? (int)(left / 32) : 4;
+            const uint32_t sfa = tmem_base + XM_BN + set * 8 * T, sfb = sfa + 4 * T;
+            const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES)), b = xm_desc_op(smem_u32(sB + stage * XM_OP_BYTES));
+            if (xm_elect()) {
 #pragma unroll
-                    for (int t = 0; t < T; t++) {
-                        if (t * (4 / T) < mmas) {
-                            xm_copy_sf(sfa + 4 * t, smem_u32(sSA + (stage * T + t) * 512));
-                            xm_copy_sf(sfb + 4 * t, smem_u32(sSB + (stage * T + t) * 512));
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (j < mmas)
-                            xm_mma<FMT>(d, xm_desc_op(a + 32 * j), xm_desc_op(b + 32 * j), xm_idesc<FMT>(XM_BN, XM_BM, j),
-                                        sfa + 4 * (j * T / 4), sfb + 4 * (j * T / 4), (kb | (uint32_t)j) != 0);
-                    }
-                    xm_commit(empty(stage));
-                    if (++stage == XM_STAGES) { stage = 0; phase ^= 1; }
+                for (int j = 0; j < 4; j++) {
+                    if (j < mmas)  // 32 bytes of k on: two units of the descriptor's address
+                        xm_mma<FMT>(tmem_base, a + 2 * j, b + 2 * j, xm_idesc<FMT>(XM_BN, XM_BM, j),
+                                    sfa + 4 * (j * T / 4), sfb + 4 * (j * T / 4), ((kb - k0) | (uint32_t)j) != 0);
                 }
-                if (ok) xm_commit(tfull(ab));
+                xm_commit(empty(stage));
+                if (kb + 1 == k1) xm_commit(done);
             }
+            __syncwarp();
+            if (++stage == S) { stage = 0; phase ^= 1; }
+            if (++set == X1_SETS) { set = 0; sphase ^= 1; }
         }
     } else {
-        const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may read
-        uint32_t local = 0;
-        for (uint64_t tile = blockIdx.x; tile < ntiles; tile += gridDim.x, local++) {
-            const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
-            if (!xm_wait(tfull(ab), aphase)) break;
-            xm_fence_after();
-            const uint64_t row = tile % tiles_m * XM_BM + quad * 32 + lane, n0 = tile / tiles_m * XM_BN;
-#pragma unroll 1
-            for (int c = 0; c < XM_BN / 32; c++) {
-                uint32_t r[32];
-                xm_ld32(tmem_base + ab * XM_BN + ((quad * 32) << 16) + c * 32, r);
-                if (row < p.m) xm_store32<TY>(C + row * p.ldc, n0 + c * 32, p.n, p.vec, p.alpha, r);
+        const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may access
+        uint32_t stage = 0, phase = 0, set = 0, old = 0, old_phase = 0;
+        for (uint32_t kb = k0; kb < k1; kb++) {
+            // the set is free once the MMAs of the step X1_SETS back, whose commit frees its stage, are done
+            if (kb - k0 >= X1_SETS) {
+                if (!xm_wait(empty(old), old_phase)) { ok = false; break; }
+                if (++old == S) { old = 0; old_phase ^= 1; }
             }
+            if (!xm_wait(full(stage), phase)) { ok = false; break; }
+            xm_fence_after();
+            const uint32_t at = tmem_base + ((quad * 32) << 16) + XM_BN + set * 8 * T;
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                x1_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(sSA + (stage * T + t) * 512 + lane * 16));
+                x1_st4(at + 4 * T + 4 * t, *reinterpret_cast<const uint4 *>(sSB + (stage * T + t) * 512 + lane * 16));
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             xm_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(tempty(ab));
+            if (lane == 0) mbar_arrive(sready(set));
+            if (++stage == S) { stage = 0; phase ^= 1; }
+            if (++set == X1_SETS) set = 0;
         }
+        if (ok) ok = xm_wait(done, 0);
+        xm_fence_after();
+        // the accumulators: straight to C, or to shared memory (the ring, whose last MMA is done) for the
+        // cluster's sum; rows of 132 floats keep a warp's 128-bit accesses apart
+        const uint32_t r = quad * 32 + lane;
+        const uint64_t row = (uint64_t)tm * XM_BM + r;
+        float *mine = reinterpret_cast<float *>(smem) + r * X1_PITCH;
+        if (ok && tm * (uint64_t)XM_BM + quad * 32 < p.m) {
+#pragma unroll 1
+            for (int c = 0; c < XM_BN / 32; c++) {
+                uint32_t v[32];
+                xm_ld32(tmem_base + ((quad * 32) << 16) + c * 32, v);
+                if (ks == 1) {
+                    if (row < p.m) xm_store32<TY>(C + row * p.ldc, (uint64_t)tn * XM_BN + c * 32, p.n, p.vec, p.alpha, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        *reinterpret_cast<uint4 *>(mine + c * 32 + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+            }
+        }
+    }
+    if (ks > 1) {
+        cluster_sync_all();
+        // this CTA's columns: 32 for ks = 4, rows over the threads' quarters
+        const uint32_t width = XM_BN / ks, rows = (uint32_t)min((uint64_t)XM_BM, p.m - tm * (uint64_t)XM_BM);
+        const uint32_t groups = width / 4;  // of four columns
+        for (uint32_t i = threadIdx.x; i < rows * groups; i += XM_THREADS) {
+            const uint32_t r = i / groups, col = rank * width + i % groups * 4;
+            const uint32_t at = smem_u32(smem) + (r * X1_PITCH + col) * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t k = 0; k < ks; k++) {
+                float4 v;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                             : "r"(mapa_shared(at, k))
+                             : "memory");
+                sum.x = __fadd_rn(sum.x, v.x);
+                sum.y = __fadd_rn(sum.y, v.y);
+                sum.z = __fadd_rn(sum.z, v.z);
+                sum.w = __fadd_rn(sum.w, v.w);
+            }
+            const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+            const uint64_t n0 = (uint64_t)tn * XM_BN + col;
+            typename MxElem<TY>::type *to = C + ((uint64_t)tm * XM_BM + r) * p.ldc + n0;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (n0 + j < p.n) to[j] = MxElem<TY>::round(__fmul_rn(p.alpha, f[j]));
+        }
+        cluster_sync_all();  // no CTA leaves while another reads its sums
     }
     xm_fence_before();
     __syncthreads();
     if (warp == 1) {
         xm_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(XM_TMEM_COLS)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(X1_TMEM_COLS)
                      : "memory");
     }
 }
@@ -305,18 +376,6 @@ LYTH_D void x2_tma2(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32
         "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
-LYTH_D void x2_tma3_own(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(dst),
-        "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-        : "memory");
-}
-LYTH_D void x2_st4(uint32_t taddr, uint4 v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y),
-                 "r"(v.z), "r"(v.w)
-                 : "memory");
-}
 template <int FMT>
 LYTH_D void x2_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
 #define LYTH_X2_MMA(KIND)                                                                                  \
@@ -355,11 +414,8 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     auto tempty = [&](int b) { return smem_u32(bars + 3 * S + 2 + b); };
     auto sready = [&](int b) { return smem_u32(bars + 3 * S + 4 + b); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t crank = cluster_ctarank();
-    uint32_t pair, npairs;
-    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(pair));
-    asm volatile("mov.u32 %0, %%nclusterid.x;" : "=r"(npairs));
+    const int warp = (int)xm_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t crank = blockIdx.x & 1, pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;  // clusters of 2 along x
     const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + X2_BN - 1) / X2_BN, ntiles = tiles_m * tiles_n;
     const uint32_t steps = (p.row_bytes + 127) / 128;
 
@@ -385,37 +441,39 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     xm_fence_before();
     cluster_sync_all();
     xm_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_base = xm_uniform(*tmem_slot);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
-            bool ok = true;
-            for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
-                const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
-                const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * X2_BN);
-                for (uint32_t kb = 0; kb < steps; kb++) {
-                    if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
-                    const uint32_t lf = mapa_shared(full(stage), 0);
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        const uint32_t lead = xm_uniform(mapa_shared(full(0), 0));  // the leader's `full` barriers
+        for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
+            const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
+            const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * X2_BN);
+            for (uint32_t kb = 0; kb < steps; kb++) {
+                if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
+                const uint32_t lf = lead + 8 * stage;
+                if (xm_elect()) {
                     mbar_expect_tx(sfull(stage), 3 * T * 512);
-                    x2_tma3_own(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
-                    x2_tma3_own(smem_u32(sSB + stage * 2 * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
+                    xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
+                    xm_tma3(smem_u32(sSB + stage * 2 * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
                     mbar_expect_tx_cluster(lf, XM_OP_BYTES + X2_B_BYTES);
                     x2_tma2(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), m0, lf);
                     x2_tma2(smem_u32(sB + stage * X2_B_BYTES), &tmB, (int)(kb * 128), n0 + X2_HALF * (int)crank, lf);
-                    if (++stage == S) { stage = 0; phase ^= 1; }
                 }
+                __syncwarp();
+                if (++stage == S) { stage = 0; phase ^= 1; }
             }
-            // Tail: every stage released by the MMA's commit, so no arrival is still on its way to
-            // this CTA's barriers when it leaves.
-            if (ok)
-                for (int s = 0; s < S; s++) {
-                    if (!xm_wait(empty(stage), phase ^ 1)) break;
-                    if (++stage == S) { stage = 0; phase ^= 1; }
-                }
         }
+        // Tail: every stage released by the MMA's commit, so no arrival is still on its way to this
+        // CTA's barriers when it leaves.
+        if (ok)
+            for (int s = 0; s < S; s++) {
+                if (!xm_wait(empty(stage), phase ^ 1)) break;
+                if (++stage == S) { stage = 0; phase ^= 1; }
+            }
     } else if (warp == 1) {
-        if (lane == 0 && crank == 0) {
+        if (crank == 0) {
             uint32_t stage = 0, phase = 0, local = 0, set = 0, sphase = 0;
             bool ok = true;
             for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
@@ -429,19 +487,22 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                     xm_fence_after();
                     const uint32_t left = p.row_bytes - kb * 128;
                     const int mmas = left < 128 ? (int)(left / 32) : 4;
-                    const uint32_t sfa = tmem_base + X2_SF_COL + set * X2<FMT>::kSetCols, sfb = sfa + 4 * T;
-                    const uint32_t a = smem_u32(sA + stage * XM_OP_BYTES), b = smem_u32(sB + stage * X2_B_BYTES);
+                    const uint32_t sfa = tmem_base + X2_SF_COL + set * X2<FMT>::kSetCols, sfb = sfa + 4 * T + shift;
+                    const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES)), b = xm_desc_op(smem_u32(sB + stage * X2_B_BYTES));
+                    if (xm_elect()) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (j < mmas)
-                            x2_mma<FMT>(d, xm_desc_op(a + 32 * j), xm_desc_op(b + 32 * j), xm_idesc<FMT>(X2_BN, 256, j),
-                                        sfa + 4 * (j * T / 4), sfb + 8 * (j * T / 4) + shift, (kb | (uint32_t)j) != 0);
+                        for (int j = 0; j < 4; j++) {
+                            if (j < mmas)
+                                x2_mma<FMT>(d, a + 2 * j, b + 2 * j, xm_idesc<FMT>(X2_BN, 256, j), sfa + 4 * (j * T / 4),
+                                            sfb + 8 * (j * T / 4), (kb | (uint32_t)j) != 0);
+                        }
+                        x2_commit(empty(stage));
+                        if (kb + 1 == steps) x2_commit(tfull(ab));
                     }
-                    x2_commit(empty(stage));
+                    __syncwarp();
                     if (++stage == S) { stage = 0; phase ^= 1; }
                     if (++set == kSets) { set = 0; sphase ^= 1; }
                 }
-                if (ok) x2_commit(tfull(ab));
             }
             // After a timed-out wait, give the stages the producers may have in flight a bounded
             // chance to land (both CTAs' copies complete on these barriers) before the pair leaves.
@@ -474,9 +535,9 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                 const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * 2 * T * 512 + lane * 16;
 #pragma unroll
                 for (int t = 0; t < T; t++) {
-                    x2_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(a + t * 512));
-                    x2_st4(at + 4 * T + 8 * t, *reinterpret_cast<const uint4 *>(b + t * 512));
-                    x2_st4(at + 4 * T + 8 * t + 4, *reinterpret_cast<const uint4 *>(b + (T + t) * 512));
+                    x1_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(a + t * 512));
+                    x1_st4(at + 4 * T + 8 * t, *reinterpret_cast<const uint4 *>(b + t * 512));
+                    x1_st4(at + 4 * T + 8 * t + 4, *reinterpret_cast<const uint4 *>(b + (T + t) * 512));
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 xm_fence_before();
@@ -587,20 +648,44 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
 }
 
 template <int FMT, int TY>
-static int xm_launch(const CUtensorMap &ta, const CUtensorMap &tb, void *c, const XmArgs &p, cudaStream_t s) {
+static int x1_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &p, cudaStream_t s) {
+    constexpr int T = Xm<FMT>::kTiles;
+    const uint32_t a_rows = p.m < 128 ? ((uint32_t)p.m + 7) / 8 * 8 : 128u;
+    CUtensorMap ta, tb, tsa, tsb;
+    if (!xm_map(&ta, a, p.row_bytes, p.m, a_rows) || !xm_map(&tb, b, p.row_bytes, p.n, XM_BN) ||
+        !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, 1))
+        return LYTH_E_UNSUPPORTED;
     static bool done[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);
     if (dev < 0 || dev >= 64 || !done[dev]) {
-        e = cudaFuncSetAttribute(mx_mma_kernel<FMT, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Xm<FMT>::kSmem);
+        e = cudaFuncSetAttribute(mx_mma1_kernel<FMT, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Xm<FMT>::kSmem);
         if (e != cudaSuccess) return status_of(e);
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const uint64_t tiles = (p.m + XM_BM - 1) / XM_BM * ((p.n + XM_BN - 1) / XM_BN);
-    const uint64_t sms = (uint64_t)device_sms();
-    const unsigned grid = (unsigned)(tiles < sms ? tiles : sms);
-    mx_mma_kernel<FMT, TY><<<grid, XM_THREADS, Xm<FMT>::kSmem, s>>>(ta, tb, static_cast<typename MxElem<TY>::type *>(c), p);
+    // shares of k: as many as keep every SM to one CTA and a share at least four steps long (a cluster's
+    // sum costs about as much as four steps)
+    const uint32_t tiles = (uint32_t)((p.m + XM_BM - 1) / XM_BM * ((p.n + XM_BN - 1) / XM_BN));
+    const uint32_t steps = (p.row_bytes + 127) / 128;
+    uint32_t ks = 1;
+    while (ks < 8 && tiles * ks * 2 <= (uint32_t)device_sms() && steps / (ks * 2) >= 4) ks *= 2;
+    if (getenv("KS")) ks = atoi(getenv("KS"));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(tiles * ks);
+    cfg.blockDim = dim3(XM_THREADS);
+    cfg.dynamicSmemBytes = Xm<FMT>::kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, mx_mma1_kernel<FMT, TY>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p,
+                           ks, a_rows);
+    if (e != cudaSuccess) return status_of(e);
     return last_launch_status();
 }
 
@@ -637,11 +722,11 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     p.words = (uint32_t)(k / (4 * mx_block(fmt)));
     p.alpha = alpha;
     p.vec = aligned32(c) && ldc * mx_ty_bytes(ty) % 32 == 0;
-    if (getenv("X2") ? atoi(getenv("X2")) : m > 128) {
+    // one tile per SM at most: single SMs, else pairs
+    const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
+    if (getenv("X2") ? atoi(getenv("X2")) : tiles > (uint64_t)device_sms()) {
         LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY>(a, b, c, p, s)));
     }
-    CUtensorMap ta, tb;
-    if (!xm_map(&ta, a, p.row_bytes, m, XM_BM) || !xm_map(&tb, b, p.row_bytes, n, XM_BN)) return LYTH_E_UNSUPPORTED;
-    LYTH_MX_DISPATCH(fmt, ty, return (xm_launch<FMT, TY>(ta, tb, c, p, s)));
+    LYTH_MX_DISPATCH(fmt, ty, return (x1_launch<FMT, TY>(a, b, c, p, s)));
     return LYTH_E_UNSUPPORTED;
 }
