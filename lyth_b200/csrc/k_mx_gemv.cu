@@ -17,9 +17,9 @@
 //                        lane each) and 16-byte asynchronous copies of the scales, completion on an
 //                        mbarrier. (One warp for all sixteen rows needed 2000 cycles to issue a stage.)
 //   consumers (16 warps) put x into shared memory as f16 once. Two teams of eight then take every other
-//                        16-row group, a warp every eighth 64-byte step of a stage, so that one team's
-//                        waits and sums lie under the other's conversions (all sixteen on one stage:
-//                        11.5 us). The partial sums of a group stay in shared memory, where all meet once
+//                        stage, a warp every eighth 64-byte step of it, so that one team's waits and sums
+//                        lie under the other's conversions (all sixteen on one stage: 11.5 us, with the
+//                        teams 10.6). The partial sums of a group stay in shared memory, where all meet once
 //                        at the end and add them up in a fixed order. Where x does not fit, k is walked
 //                        in chunks, x staged chunk by chunk.
 // Every mbarrier wait is bounded (mbar.cuh); one that runs out sets the device error flag and the
@@ -38,7 +38,7 @@ namespace lyth {
 __device__ int g_xv_error = 0;
 
 constexpr int XV_WARPS = 16;                        // consumers
-constexpr int XV_TEAM = XV_WARPS / 2;               // a team takes every other group
+constexpr int XV_TEAM = XV_WARPS / 2;               // a team takes every other stage
 constexpr int XV_PRODUCERS = 4;                     // warps, one per quad of a group
 constexpr int XV_THREADS = 32 * (XV_WARPS + XV_PRODUCERS);
 constexpr int XV_SEG = 2048;                        // bytes of a row in a stage
@@ -66,7 +66,7 @@ struct XvArgs {
     uint32_t quads_each, quads_more;  // quads of a block; blocks that have one more
     uint32_t row_bytes, words;        // bytes of a row of codes; scale words along k
     uint32_t segs;                    // stages along k
-    uint32_t chunk;                   // segments whose x is in shared memory at once
+    uint32_t chunk, xsteps;           // segments, and steps, whose x is in shared memory at once
     uint32_t stages;                  // of the ring
     float alpha;
     bool vec;                         // rows of x start on 16 bytes
@@ -142,7 +142,15 @@ LYTH_D uint4 xv_f16(uint4 u, float scale) {
 }
 
 LYTH_D void xv_sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * XV_WARPS) : "memory"); }
-LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) { return mbar_wait(bar, parity, &g_xv_error); }
+// Warps wait together and decide by vote, so what follows is uniform control flow.
+LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, &g_xv_error));
+}
+LYTH_D bool xv_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 
 // Where a block is in its walk: batches of groups, chunks of k, groups, segments. All roles take the
 // same steps.
@@ -249,10 +257,10 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     extern __shared__ __align__(128) uint8_t sm[];        // ring, x, partial sums
     __shared__ uint64_t bars[2 * 4 + 1];
     __shared__ uint32_t s_max[XV_WARPS];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t xunits = p.chunk * XV_STEPS * 4 * kUnits;  // 16-byte units of x per token
+    const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t xunits = p.xsteps * 4 * kUnits;        // 16-byte units of x per token
     uint4 *sx = reinterpret_cast<uint4 *>(sm + p.stages * Xv<FMT>::kStage);
-    float *s_part = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // [group][warp of its team][token][row]
+    float *s_part = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // [group][warp][token][row]
     auto full = [&](uint32_t s) { return smem_u32(bars + s); };
     auto empty = [&](uint32_t s) { return smem_u32(bars + 4 + s); };
     const uint32_t xbar = smem_u32(bars + 8);             // the consumers' meeting point
@@ -275,24 +283,29 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             for (uint32_t c0 = 0; ok && c0 < p.segs; c0 += p.chunk) {
                 const uint32_t c1 = min(c0 + p.chunk, p.segs);
                 for (uint32_t group = 0; ok && group < w.groups; group++) {
-                    // a warp per quad: lane j < 4 brings the row of quarter j, all lanes its scale words
-                    const uint32_t quad = w.lo + 4 * group + (warp - XV_WARPS), row = xv_row(quad, lane & 3);
-                    const bool has = quad < w.hi, has_row = lane < 4 && has && row <= w.last;
-                    const uint32_t rows = __popc(__ballot_sync(0xFFFFFFFFu, has_row));
+                    // a warp per quad: one lane brings its four rows, all lanes its scale words
+                    const uint32_t pw = warp - XV_WARPS, quad = w.lo + 4 * group + pw, row = xv_row(quad, 0);
+                    const bool has = quad < w.hi;
+                    const uint32_t rows = !has || row > w.last ? 0u : min((w.last - row) / 32 + 1, 4u);
                     const uint8_t *src = w_base + (uint64_t)row * p.row_bytes;
                     const uint8_t *ssrc = s_base + (uint64_t)(quad >> 5) * p.words * 512 + (quad & 31) * 16;
                     for (uint32_t seg = c0; seg < c1; seg++) {
                         if (!xv_wait(empty(stage), phase ^ 1)) { ok = false; break; }
                         const uint32_t bytes = min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG);
                         const uint32_t at = smem_u32(sm) + stage * Xv<FMT>::kStage;
-                        if (lane == 0) mbar_expect_tx(full(stage), rows * bytes);
+                        if (xv_elect()) {
+                            mbar_expect_tx(full(stage), rows * bytes);
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++)
+                                if (j < rows)
+                                    bulk_load(at + (pw * 4 + j) * XV_ROW, src + seg * XV_SEG + (uint64_t)j * 32 * p.row_bytes, bytes,
+                                              full(stage));
+                        }
                         __syncwarp();
-                        if (has_row)
-                            bulk_load(at + ((warp - XV_WARPS) * 4 + lane) * XV_ROW, src + seg * XV_SEG, bytes, full(stage));
                         const uint32_t w0 = seg * Xv<FMT>::kWords, nw = min(p.words - w0, (uint32_t)Xv<FMT>::kWords);
                         if (has)
                             for (uint32_t i = lane; i < nw; i += 32)
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + XV_W_BYTES + i * 64 + (warp - XV_WARPS) * 16),
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + XV_W_BYTES + i * 64 + pw * 16),
                                              "l"(ssrc + (uint64_t)(w0 + i) * 512)
                                              : "memory");
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(stage)) : "memory");
@@ -323,13 +336,28 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             x_at[pr] = smem_u32(sx + min(2u * pr + (g >> 2), p.m - 1) * (xunits + 4) + t);
         const T *x = static_cast<const T *>(p.x);
         float scale = 1.0f;
-        // (rolled loops: code that runs once is fetched from memory as it runs)
+        // Units of x, token after token, four of a thread's loads in flight; `per` units of a token from
+        // unit `first` on.
+        auto each = [&](uint32_t first, uint32_t per, auto &&use) {
+#pragma unroll 1
+            for (uint32_t i0 = threadIdx.x; i0 < p.m * per; i0 += 4 * 32 * XV_WARPS) {
+                uint4 v[4];
+                uint32_t tok[4], u[4];
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    const uint32_t i = i0 + h * 32 * XV_WARPS;
+                    tok[h] = p.m == 1 ? 0u : i / per;
+                    u[h] = i - tok[h] * per;
+                    if (i < p.m * per) v[h] = xv_load8<TY>(x + tok[h] * p.ldx, 8 * (first + u[h]), p.cols, p.vec);
+                }
+#pragma unroll
+                for (int h = 0; h < 4; h++)
+                    if (i0 + h * 32 * XV_WARPS < p.m * per) use(tok[h], u[h], v[h]);
+            }
+        };
         if constexpr (TY == LYTH_NARROW_BF16) {
             uint32_t top = 0;
-            for (uint32_t tok = 0; tok < p.m; tok++)
-#pragma unroll 1
-                for (uint32_t u = threadIdx.x; u < (p.cols + 7) / 8; u += 32 * XV_WARPS)
-                    top = max(top, xv_top(xv_load8<TY>(x + tok * p.ldx, 8 * u, p.cols, p.vec)));
+            each(0, (p.cols + 7) / 8, [&](uint32_t, uint32_t, uint4 v) { top = max(top, xv_top(v)); });
             top = __reduce_max_sync(0xFFFFFFFFu, top);
             if (lane == 0) s_max[warp] = top;
             xv_sync_consumers();
@@ -339,7 +367,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             scale = __uint_as_float((uint32_t)(sh + 127) << 23);
         }
         const float unscale = __uint_as_float((254u << 23) - __float_as_uint(scale));
-        uint32_t stage = 0, phase = 0;
+        uint32_t stage = 0, phase = 0, turn = 1;
         bool ok = true, staged = false;
         uint32_t xphase = 0;
         auto meet = [&]() {
@@ -356,25 +384,22 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                     // (a bounded meeting: a warp that gave up a wait has left)
                     if (staged && !(ok = meet())) break;
                     const uint32_t first = c0 * XV_STEPS * 4 * kUnits;
-                    for (uint32_t tok = 0; tok < p.m; tok++)
-#pragma unroll 1
-                        for (uint32_t u = threadIdx.x; u < xunits; u += 32 * XV_WARPS) {
-                            const uint32_t at = u / (4 * kUnits) * (4 * kUnits) + u % kUnits * 4 + u / kUnits % 4;
-                            sx[tok * (xunits + 4) + at] =
-                                xv_f16<TY>(xv_load8<TY>(x + tok * p.ldx, 8 * (first + u), p.cols, p.vec), scale);
-                        }
+                    each(first, xunits, [&](uint32_t tok, uint32_t u, uint4 v) {
+                        const uint32_t at = u / (4 * kUnits) * (4 * kUnits) + u % kUnits * 4 + u / kUnits % 4;
+                        sx[tok * (xunits + 4) + at] = xv_f16<TY>(v, scale);
+                    });
                     if (!(ok = meet())) break;
                     staged = true;
                 }
                 const uint32_t c1 = min(c0 + p.chunk, p.segs);
                 for (uint32_t group = 0; ok && group < w.groups; group++) {
-                    if ((group & 1) != warp / XV_TEAM) {  // the other team's
-                        for (uint32_t seg = c0; seg < c1; seg++)
-                            if (++stage == p.stages) { stage = 0; phase ^= 1; }
-                        continue;
-                    }
                     float acc[PAIRS][2] = {};
                     for (uint32_t seg = c0; seg < c1; seg++) {
+                        turn ^= 1;
+                        if (turn != warp / XV_TEAM) {  // the other team's stage
+                            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                            continue;
+                        }
                         if (!xv_wait(full(stage), phase)) { ok = false; break; }
                         const uint8_t *at = sm + stage * Xv<FMT>::kStage;
                         const uint32_t steps = (min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG) + 63) / 64;
@@ -391,7 +416,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                     }
                     if (!ok) break;
                     // this warp's part of the group, of its own from chunk to chunk
-                    float *part = s_part + (group * XV_TEAM + warp % XV_TEAM) * (kTokens * 16);
+                    float *part = s_part + (group * XV_WARPS + warp) * (kTokens * 16);
 #pragma unroll
                     for (int pr = 0; pr < PAIRS; pr++)
 #pragma unroll
@@ -407,10 +432,10 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             for (uint32_t i = threadIdx.x; i < w.groups * p.m * 16; i += 32 * XV_WARPS) {
                 const uint32_t group = i / 16 % w.groups, tok = i / 16 / w.groups, r = i & 15;
                 const uint32_t quad = w.lo + 4 * group + (r >> 2), row = xv_row(quad, r & 3);
-                const float *part = s_part + (group * XV_TEAM * kTokens + tok) * 16 + r;
+                const float *part = s_part + (group * XV_WARPS * kTokens + tok) * 16 + r;
                 float v = 0.0f;
 #pragma unroll
-                for (int k = 0; k < XV_TEAM; k++) v = __fadd_rn(v, part[k * kTokens * 16]);
+                for (int k = 0; k < XV_WARPS; k++) v = __fadd_rn(v, part[k * kTokens * 16]);
                 if (quad < w.hi && row <= w.last)
                     static_cast<T *>(p.y)[tok * p.ldy + w.tile0 * 128 + row] =
                         MxElem<TY>::round(__fmul_rn(p.alpha, __fmul_rn(v, unscale)));
@@ -422,16 +447,23 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
 
 template <int FMT, int TY, int PAIRS>
 static int xv_launch(XvArgs p, cudaStream_t s) {
-    // Shared memory: the partial sums, a ring of 3 or 4 stages, and as many segments of x as are left
-    // room for (at least one: 8 tokens x 2048 E2M1 bytes are 64 KiB).
-    const size_t seg_x = (size_t)p.m * XV_STEPS * (FMT == LYTH_MX_FP8 ? 8 : 16) * 16;
-    const size_t fixed = (size_t)kXvBatch<PAIRS> * XV_TEAM * 2 * PAIRS * 16 * sizeof(float) + p.m * 64;
-    const size_t room = 226 * 1024 - fixed;
+    const uint32_t quads = p.n / 128 * 32 + (p.n % 128 < 32 ? p.n % 128 : 32u);
+    const uint32_t sms = (uint32_t)device_sms(), grid = quads < sms ? quads : sms;
+    p.quads_each = quads / grid;
+    p.quads_more = quads % grid;
+    // Shared memory: the partial sums, a ring of 3 or 4 stages, and as much of x as there is room for (at
+    // least a segment: 8 tokens x 2048 E2M1 bytes are 64 KiB).
+    const uint32_t groups = (p.quads_each + (p.quads_more ? 1 : 0) + 3) / 4;
+    const size_t sums = (size_t)(groups < (uint32_t)kXvBatch<PAIRS> ? groups : kXvBatch<PAIRS>) * XV_WARPS * 2 * PAIRS * 16 * sizeof(float);
+    const size_t step_x = (size_t)p.m * (FMT == LYTH_MX_FP8 ? 8 : 16) * 16;
+    const uint32_t steps = (p.row_bytes + 63) / 64;
+    const size_t room = 226 * 1024 - sums - p.m * 64;
     p.stages = 4;
-    if (4 * (size_t)Xv<FMT>::kStage + p.segs * seg_x > room) p.stages = 3;
-    const size_t most = (room - p.stages * (size_t)Xv<FMT>::kStage) / seg_x;
-    p.chunk = p.segs < most ? p.segs : (uint32_t)most;
-    const size_t smem = p.stages * (size_t)Xv<FMT>::kStage + p.chunk * seg_x + fixed;
+    if (4 * (size_t)Xv<FMT>::kStage + steps * step_x > room) p.stages = 3;
+    const size_t x_room = room - p.stages * (size_t)Xv<FMT>::kStage;
+    p.chunk = steps * step_x <= x_room ? p.segs : (uint32_t)(x_room / (XV_STEPS * step_x));
+    p.xsteps = p.chunk == p.segs ? steps : p.chunk * XV_STEPS;
+    const size_t smem = p.stages * (size_t)Xv<FMT>::kStage + p.xsteps * step_x + p.m * 64 + sums;
     static size_t set[64] = {0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -441,10 +473,6 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
         if (e != cudaSuccess) return status_of(e);
         if (dev >= 0 && dev < 64) set[dev] = 1;
     }
-    const uint32_t quads = p.n / 128 * 32 + (p.n % 128 < 32 ? p.n % 128 : 32u);
-    const uint32_t sms = (uint32_t)device_sms(), grid = quads < sms ? quads : sms;
-    p.quads_each = quads / grid;
-    p.quads_more = quads % grid;
     mx_gemv_kernel<FMT, TY, PAIRS><<<grid, XV_THREADS, smem, s>>>(p);
     return last_launch_status();
 }

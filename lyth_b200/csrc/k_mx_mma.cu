@@ -3,19 +3,14 @@
 // f16 or bf16. tcgen05.mma .block_scale multiplies the codes and applies both operands' block scales
 // inside the contraction, so nothing is dequantised.
 //
-// One persistent CTA per SM, 192 threads, warp-specialised as the bf16 contraction (k_mma.cu):
-//   warp 0     producer: per step of 128 bytes along k (128 E4M3 or 256 E2M1 codes), a 128-row box of
-//              A and of B (128-byte swizzle) and both operands' scale tiles (512 bytes per 128 rows x
-//              4 blocks, already in the order tensor memory wants) into a ring.
-//   warp 1     one thread copies the step's scale tiles to tensor memory (tcgen05.cp 32x128b, spread to
-//              the four lane quadrants) and issues one MMA per 32 bytes of k; tcgen05.cp and
-//              tcgen05.mma of one thread run in order, so the scales need no wait of their own.
-//   warps 2-5  epilogue: tcgen05.ld, times alpha, rounded once, stored; two accumulators let it run
-//              beside the next tile's main loop.
+// Two forms, chosen by the number of 128 x 128 tiles: up to one per SM, single SMs whose clusters share k
+// (mx_mma1_kernel); more, CTA pairs on 256 x 192 tiles (mx_mma2_kernel). Both stage steps of 128 bytes
+// along k (128 E4M3 or 256 E2M1 codes) of A and B in a shared-memory ring (TMA, 128-byte swizzle, no
+// multicast) with both operands' scale tiles (512 bytes per 128 rows x 4 blocks, already in the order
+// tensor memory wants), move the scales to tensor memory and issue one MMA per 32 bytes of k.
 // Ragged edges: rows behind m or n arrive as zeros (tensor-map fill) or carry any scale, and are not
 // stored; k is whole scale words, so the last step's MMAs are only fewer. Every wait is bounded.
 #include <cuda.h>
-#include <stdlib.h>
 
 #include "mbar.cuh"
 #include "mx.cuh"
@@ -670,7 +665,6 @@ static int x1_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     const uint32_t steps = (p.row_bytes + 127) / 128;
     uint32_t ks = 1;
     while (ks < 8 && tiles * ks * 2 <= (uint32_t)device_sms() && steps / (ks * 2) >= 4) ks *= 2;
-    if (getenv("KS")) ks = atoi(getenv("KS"));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -724,7 +718,7 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     p.vec = aligned32(c) && ldc * mx_ty_bytes(ty) % 32 == 0;
     // one tile per SM at most: single SMs, else pairs
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
-    if (getenv("X2") ? atoi(getenv("X2")) : tiles > (uint64_t)device_sms()) {
+    if (tiles > (uint64_t)device_sms()) {
         LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY>(a, b, c, p, s)));
     }
     LYTH_MX_DISPATCH(fmt, ty, return (x1_launch<FMT, TY>(a, b, c, p, s)));
