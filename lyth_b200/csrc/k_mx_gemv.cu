@@ -142,15 +142,7 @@ LYTH_D uint4 xv_f16(uint4 u, float scale) {
 }
 
 LYTH_D void xv_sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * XV_WARPS) : "memory"); }
-// Warps wait together and decide by vote, so what follows is uniform control flow.
-LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, &g_xv_error));
-}
-LYTH_D bool xv_elect() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0;
-}
+LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, &g_xv_error); }
 
 // Where a block is in its walk: batches of groups, chunks of k, groups, segments. All roles take the
 // same steps.
@@ -257,7 +249,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     extern __shared__ __align__(128) uint8_t sm[];        // ring, x, partial sums
     __shared__ uint64_t bars[2 * 4 + 1];
     __shared__ uint32_t s_max[XV_WARPS];
-    const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t xunits = p.xsteps * 4 * kUnits;        // 16-byte units of x per token
     uint4 *sx = reinterpret_cast<uint4 *>(sm + p.stages * Xv<FMT>::kStage);
     float *s_part = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // [group][warp][token][row]
@@ -293,7 +285,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                         if (!xv_wait(empty(stage), phase ^ 1)) { ok = false; break; }
                         const uint32_t bytes = min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG);
                         const uint32_t at = smem_u32(sm) + stage * Xv<FMT>::kStage;
-                        if (xv_elect()) {
+                        if (elect_one()) {
                             mbar_expect_tx(full(stage), rows * bytes);
 #pragma unroll
                             for (uint32_t j = 0; j < 4; j++)

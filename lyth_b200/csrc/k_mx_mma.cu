@@ -19,7 +19,7 @@ namespace lyth {
 
 __device__ int g_mx_error = 0;
 
-constexpr int XM_BM = 128, XM_BN = 128, XM_STAGES = 6, XM_THREADS = 192;
+constexpr int XM_BM = 128, XM_BN = 128, XM_STAGES = 6;
 constexpr int XM_OP_BYTES = 128 * 128;         // one operand's box: 128 rows x 128 bytes
 constexpr int XM_TMEM_COLS = 512;              // the pair form: two accumulators, then the scales
 constexpr int X1_TMEM_COLS = 256;              // the single-SM form: an accumulator, then the scales
@@ -49,15 +49,10 @@ LYTH_D uint32_t xm_idesc(int n, int m, int j) {
 // lane issues. The operands of TMA and MMA instructions then stay in uniform registers; a loop of a
 // single lane (`if (lane == 0)`) had the compiler gather them for each instruction, 880 cycles for the
 // four MMAs and two waits of a step and 550 for its four copies, which bound the kernels.
-LYTH_D bool xm_wait(uint32_t bar, uint32_t parity) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, &g_mx_error));
+LYTH_D bool xm_wait(uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, &g_mx_error); }
+LYTH_D void xm_prefetch(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory");
 }
-LYTH_D bool xm_elect() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0;
-}
-LYTH_D uint32_t xm_uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
 
 // Shared-memory descriptor: K-major rows of 128 bytes with the 128-byte swizzle (8-row groups 1024
 // bytes apart).
@@ -110,41 +105,57 @@ struct XmArgs {
     bool vec;                // rows of C start on 32 bytes
 };
 
-// 32 accumulators of one row to C, columns col .. col + 31: in 256-bit stores, a whole sector each,
-// where rows start on 32 bytes.
+// A warp's 32 x 32 accumulators (a row a lane) to C, rows row0 .. row0 + 31, columns col .. col + 31.
+// Rows that start on 32 bytes are stored by their lanes in 256-bit pieces, whole sectors; others go
+// through `turn`, the warp's 32 x 17 floats of shared memory, sixteen columns at a time, so that sixteen
+// lanes store a row's neighbouring elements (1001 x 1111 f32, stored by lanes of different rows: 25 us of
+// a product that now takes 10).
+constexpr int XM_TURN = 32 * 17;
 template <int TY>
-LYTH_D void xm_store32(typename MxElem<TY>::type *crow, uint64_t col, uint64_t n, bool vec, float alpha,
+LYTH_D void xm_store32(typename MxElem<TY>::type *C, uint64_t row0, uint64_t col, const XmArgs &p, float *turn,
                        const uint32_t (&r)[32]) {
-    if (col >= n) return;
-    const uint32_t left = n - col < 32 ? (uint32_t)(n - col) : 32u;
+    if (col >= p.n) return;
+    const uint32_t lane = threadIdx.x & 31, left = p.n - col < 32 ? (uint32_t)(p.n - col) : 32u;
+    const uint32_t rows = p.m - row0 < 32 ? (uint32_t)(p.m - row0) : 32u;
 #pragma unroll
     for (int v = 0; v < 2; v++) {
         float f[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) f[i] = __fmul_rn(alpha, __uint_as_float(r[16 * v + i]));
-        if (vec && 16u * v + 16 <= left) {
-            uint32_t w[kMxWords<TY>];
-            mx_narrow<TY>(f, w);
+        for (int i = 0; i < 16; i++) f[i] = __fmul_rn(p.alpha, __uint_as_float(r[16 * v + i]));
+        if (p.vec && 16u * v + 16 <= left) {
+            if (lane < rows) {
+                uint32_t w[kMxWords<TY>];
+                mx_narrow<TY>(f, w);
+                uint32_t *to = reinterpret_cast<uint32_t *>(C + (row0 + lane) * p.ldc + col + 16 * v);
 #pragma unroll
-            for (int i = 0; i < kMxWords<TY>; i += 8) mx_st32(reinterpret_cast<uint32_t *>(crow + col + 16 * v) + i, w + i);
+                for (int i = 0; i < kMxWords<TY>; i += 8) mx_st32(to + i, w + i);
+            }
         } else {
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (16u * v + i < left) crow[col + 16 * v + i] = MxElem<TY>::round(f[i]);
+            for (int i = 0; i < 16; i++) turn[lane * 17 + i] = f[i];
+            __syncwarp();
+            const uint32_t c = lane & 15;
+            typename MxElem<TY>::type *to = C + row0 * p.ldc + col + 16 * v + c;
+            if (16u * v + c < left) {
+#pragma unroll 4
+                for (uint32_t i = lane >> 4; i < rows; i += 2) to[(uint64_t)i * p.ldc] = MxElem<TY>::round(turn[i * 17 + c]);
+            }
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// The single-SM form, for products of at most one 128 x 128 tile per SM: a cluster of KS CTAs (1, 2, 4
-// or 8) takes a tile, each a contiguous share of k, so that few tiles still fill the machine; their
+// The single-SM form, for products of at most one 128 x 128 tile per SM: a cluster of 1, 2 or 4 CTAs
+// takes a tile, each a contiguous share of k, so that few tiles still fill the machine; their
 // accumulators meet in shared memory and every CTA adds up a share of the columns over the cluster, in
 // rank order. One token batch of 32 through 14336 x 4096 is 112 tiles; through 4096 x 14336, 32 tiles
 // of four shares.
 //   warp 0     producer: boxes of A (only the rows that exist), B and both operands' scales.
 //   warp 1     issues the MMAs.
-//   warps 2-5  scales from shared to tensor memory as below, then the epilogue.
-constexpr int X1_SETS = 4;
+//   warps 2-9  scales from shared to tensor memory as below, four warps the even steps and four the odd
+//              (a step takes one set of four 600 cycles, the MMAs of it 260), then the epilogue.
+constexpr int X1_SETS = 4, X1_THREADS = 320;
 
 LYTH_D void x1_st4(uint32_t taddr, uint4 v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y),
@@ -160,10 +171,10 @@ LYTH_D void xm_tma3(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2
 }
 
 template <int FMT, int TY>
-__global__ void __launch_bounds__(XM_THREADS, 1)
+__global__ void __launch_bounds__(X1_THREADS, 1)
     mx_mma1_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                   typename MxElem<TY>::type *C, XmArgs p, uint32_t ks, uint32_t a_rows) {
+                   typename MxElem<TY>::type *C, XmArgs p, uint32_t klog, uint32_t a_rows) {
     constexpr int T = Xm<FMT>::kTiles, S = XM_STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -175,17 +186,23 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
     auto sready = [&](int b) { return smem_u32(bars + 2 * S + b); };
     const uint32_t done = smem_u32(bars + 2 * S + X1_SETS);
 
-    const int warp = (int)xm_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x % ks, tile = blockIdx.x / ks;
+    const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint32_t ks = 1u << klog, rank = blockIdx.x & (ks - 1), tile = blockIdx.x >> klog;
     const uint32_t tiles_m = (uint32_t)((p.m + XM_BM - 1) / XM_BM), tm = tile % tiles_m, tn = tile / tiles_m;
     const uint32_t all = (p.row_bytes + 127) / 128, k0 = all * rank / ks, k1 = all * (rank + 1) / ks;
 
+    if (threadIdx.x == 32) {
+        xm_prefetch(&tmA);
+        xm_prefetch(&tmB);
+        xm_prefetch(&tmSA);
+        xm_prefetch(&tmSB);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        for (int b = 0; b < X1_SETS; b++) mbar_init(sready(b), 4);
+        for (int b = 0; b < X1_SETS; b++) mbar_init(sready(b), 4);  // the four warps of the step
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -198,14 +215,14 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
     xm_fence_before();
     __syncthreads();
     xm_fence_after();
-    const uint32_t tmem_base = xm_uniform(*tmem_slot);
+    const uint32_t tmem_base = warp_uniform(*tmem_slot);
     bool ok = true;
 
     if (warp == 0) {
         uint32_t stage = 0, phase = 0;
         for (uint32_t kb = k0; kb < k1; kb++) {
             if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
-            if (xm_elect()) {
+            if (elect_one()) {
                 mbar_expect_tx(full(stage), a_rows * 128 + XM_OP_BYTES + 2 * T * 512);
                 xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), (int)tm, full(stage));
                 xm_tma3(smem_u32(sSB + stage * T * 512), &tmSB, 0, (int)(kb * T), (int)tn, full(stage));
@@ -226,13 +243,14 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
     } else if (warp == 1) {
         uint32_t stage = 0, phase = 0, set = 0, sphase = 0;
         for (uint32_t kb = k0; kb < k1; kb++) {
-            if (!xm_wait(full(stage), phase) || !xm_wait(sready(set), sphase)) { ok = false; break; }
+            // the scale warps have seen this step's copies land (`full`) before they arrive here
+            if (!xm_wait(sready(set), sphase)) { ok = false; break; }
             xm_fence_after();
             const uint32_t left = p.row_bytes - kb * 128;
             const int mmas = left < 128 ? (int)(left / 32) : 4;
             const uint32_t sfa = tmem_base + XM_BN + set * 8 * T, sfb = sfa + 4 * T;
             const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES)), b = xm_desc_op(smem_u32(sB + stage * XM_OP_BYTES));
-            if (xm_elect()) {
+            if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if (j < mmas)  // 32 bytes of k on: two units of the descriptor's address
@@ -248,12 +266,13 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
         }
     } else {
         const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may access
-        uint32_t stage = 0, phase = 0, set = 0, old = 0, old_phase = 0;
-        for (uint32_t kb = k0; kb < k1; kb++) {
+        const uint32_t half = (uint32_t)(warp - 2) >> 2;  // of the steps, then of the columns
+        uint32_t stage = half, phase = 0, set = half, old = half, old_phase = 0;
+        for (uint32_t kb = k0 + half; kb < k1; kb += 2) {
             // the set is free once the MMAs of the step X1_SETS back, whose commit frees its stage, are done
             if (kb - k0 >= X1_SETS) {
                 if (!xm_wait(empty(old), old_phase)) { ok = false; break; }
-                if (++old == S) { old = 0; old_phase ^= 1; }
+                if ((old += 2) >= S) { old -= S; old_phase ^= 1; }
             }
             if (!xm_wait(full(stage), phase)) { ok = false; break; }
             xm_fence_after();
@@ -267,23 +286,23 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
             xm_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(sready(set));
-            if (++stage == S) { stage = 0; phase ^= 1; }
-            if (++set == X1_SETS) set = 0;
+            if ((stage += 2) >= S) { stage -= S; phase ^= 1; }
+            if ((set += 2) >= X1_SETS) set -= X1_SETS;
         }
         if (ok) ok = xm_wait(done, 0);
         xm_fence_after();
         // the accumulators: straight to C, or to shared memory (the ring, whose last MMA is done) for the
         // cluster's sum; rows of 132 floats keep a warp's 128-bit accesses apart
         const uint32_t r = quad * 32 + lane;
-        const uint64_t row = (uint64_t)tm * XM_BM + r;
         float *mine = reinterpret_cast<float *>(smem) + r * X1_PITCH;
         if (ok && tm * (uint64_t)XM_BM + quad * 32 < p.m) {
 #pragma unroll 1
-            for (int c = 0; c < XM_BN / 32; c++) {
+            for (uint32_t c = 2 * half; c < 2 * half + 2; c++) {
                 uint32_t v[32];
                 xm_ld32(tmem_base + ((quad * 32) << 16) + c * 32, v);
                 if (ks == 1) {
-                    if (row < p.m) xm_store32<TY>(C + row * p.ldc, (uint64_t)tn * XM_BN + c * 32, p.n, p.vec, p.alpha, v);
+                    xm_store32<TY>(C, (uint64_t)tm * XM_BM + quad * 32, (uint64_t)tn * XM_BN + c * 32, p,
+                                   reinterpret_cast<float *>(smem) + (warp - 2) * XM_TURN, v);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; i++)
@@ -294,30 +313,43 @@ __global__ void __launch_bounds__(XM_THREADS, 1)
     }
     if (ks > 1) {
         cluster_sync_all();
-        // this CTA's columns: 32 for ks = 4, rows over the threads' quarters
-        const uint32_t width = XM_BN / ks, rows = (uint32_t)min((uint64_t)XM_BM, p.m - tm * (uint64_t)XM_BM);
-        const uint32_t groups = width / 4;  // of four columns
-        for (uint32_t i = threadIdx.x; i < rows * groups; i += XM_THREADS) {
-            const uint32_t r = i / groups, col = rank * width + i % groups * 4;
-            const uint32_t at = smem_u32(smem) + (r * X1_PITCH + col) * 4;
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (uint32_t k = 0; k < ks; k++) {
-                float4 v;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                             : "r"(mapa_shared(at, k))
-                             : "memory");
-                sum.x = __fadd_rn(sum.x, v.x);
-                sum.y = __fadd_rn(sum.y, v.y);
-                sum.z = __fadd_rn(sum.z, v.z);
-                sum.w = __fadd_rn(sum.w, v.w);
-            }
-            const float f[4] = {sum.x, sum.y, sum.z, sum.w};
-            const uint64_t n0 = (uint64_t)tn * XM_BN + col;
-            typename MxElem<TY>::type *to = C + ((uint64_t)tm * XM_BM + r) * p.ldc + n0;
+        // this CTA's columns of the sum, over the cluster in rank order
+        const uint32_t width = XM_BN >> klog, rows = (uint32_t)min((uint64_t)XM_BM, p.m - tm * (uint64_t)XM_BM);
+        const uint32_t glog = 5 - klog, items = rows << glog;  // four columns an item
+        // eight loads of a thread in flight: 8 / ks items from each of the ks CTAs
+        for (uint32_t i0 = threadIdx.x; i0 < items; i0 += X1_THREADS << (3 - klog)) {
+            float4 v[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (n0 + j < p.n) to[j] = MxElem<TY>::round(__fmul_rn(p.alpha, f[j]));
+            for (uint32_t q = 0; q < 8; q++) {
+                const uint32_t i = i0 + (q >> klog) * X1_THREADS;
+                if (i < items) {
+                    const uint32_t at = smem_u32(smem) + ((i >> glog) * X1_PITCH + rank * width + (i & ((1u << glog) - 1)) * 4) * 4;
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                                 : "r"(mapa_shared(at, q & (ks - 1)))
+                                 : "memory");
+                }
+            }
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t q = 0; q < 8; q++) {
+                sum.x = __fadd_rn(sum.x, v[q].x);
+                sum.y = __fadd_rn(sum.y, v[q].y);
+                sum.z = __fadd_rn(sum.z, v[q].z);
+                sum.w = __fadd_rn(sum.w, v[q].w);
+                if ((q & (ks - 1)) == ks - 1) {
+                    const uint32_t i = i0 + (q >> klog) * X1_THREADS;
+                    if (i < items) {
+                        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+                        const uint64_t n0 = (uint64_t)tn * XM_BN + rank * width + (i & ((1u << glog) - 1)) * 4;
+                        typename MxElem<TY>::type *to = C + ((uint64_t)tm * XM_BM + (i >> glog)) * p.ldc + n0;
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (n0 + j < p.n) to[j] = MxElem<TY>::round(__fmul_rn(p.alpha, f[j]));
+                    }
+                    sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            }
         }
         cluster_sync_all();  // no CTA leaves while another reads its sums
     }
@@ -360,8 +392,9 @@ struct X2 {
     static constexpr int kStageBytes = XM_OP_BYTES + X2_B_BYTES + 3 * kTiles * 512;
     static constexpr int kSetCols = 12 * kTiles;                     // a step's scales in tensor memory
     static constexpr int kSets = 128 / kSetCols < 4 ? 128 / kSetCols : 4;
-    static constexpr int kStages = 225 * 1024 / kStageBytes;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + 256;
+    static constexpr int kTurnBytes = 4 * XM_TURN * 4;               // the epilogue's, at 256 bytes past the ring
+    static constexpr int kStages = (227 * 1024 - 1280 - kTurnBytes) / kStageBytes;
+    static constexpr size_t kSmem = 1280 + (size_t)kStages * kStageBytes + kTurnBytes;
 };
 
 LYTH_D void x2_tma2(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
@@ -409,11 +442,17 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     auto tempty = [&](int b) { return smem_u32(bars + 3 * S + 2 + b); };
     auto sready = [&](int b) { return smem_u32(bars + 3 * S + 4 + b); };
 
-    const int warp = (int)xm_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t crank = blockIdx.x & 1, pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;  // clusters of 2 along x
     const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + X2_BN - 1) / X2_BN, ntiles = tiles_m * tiles_n;
     const uint32_t steps = (p.row_bytes + 127) / 128;
 
+    if (threadIdx.x == 32) {
+        xm_prefetch(&tmA);
+        xm_prefetch(&tmB);
+        xm_prefetch(&tmSA);
+        xm_prefetch(&tmSB);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) {
             mbar_init(full(s), 2);  // the two producers' arrivals (the leader's barrier is the one used)
@@ -436,19 +475,19 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     xm_fence_before();
     cluster_sync_all();
     xm_fence_after();
-    const uint32_t tmem_base = xm_uniform(*tmem_slot);
+    const uint32_t tmem_base = warp_uniform(*tmem_slot);
 
     if (warp == 0) {
         uint32_t stage = 0, phase = 0;
         bool ok = true;
-        const uint32_t lead = xm_uniform(mapa_shared(full(0), 0));  // the leader's `full` barriers
+        const uint32_t lead = warp_uniform(mapa_shared(full(0), 0));  // the leader's `full` barriers
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
             const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
             const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * X2_BN);
             for (uint32_t kb = 0; kb < steps; kb++) {
                 if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
                 const uint32_t lf = lead + 8 * stage;
-                if (xm_elect()) {
+                if (elect_one()) {
                     mbar_expect_tx(sfull(stage), 3 * T * 512);
                     xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
                     xm_tma3(smem_u32(sSB + stage * 2 * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
@@ -484,7 +523,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                     const int mmas = left < 128 ? (int)(left / 32) : 4;
                     const uint32_t sfa = tmem_base + X2_SF_COL + set * X2<FMT>::kSetCols, sfb = sfa + 4 * T + shift;
                     const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES)), b = xm_desc_op(smem_u32(sB + stage * X2_B_BYTES));
-                    if (xm_elect()) {
+                    if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             if (j < mmas)
@@ -545,17 +584,18 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     } else {
         const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may read
         const uint32_t lead_tempty[2] = {mapa_shared(tempty(0), 0), mapa_shared(tempty(1), 0)};
+        float *turn = reinterpret_cast<float *>(bars + 32) + quad * XM_TURN;
         uint32_t local = 0;
         for (uint64_t tile = pair; tile < ntiles; tile += npairs, local++) {
             const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
             if (!xm_wait(tfull(ab), aphase)) break;
             xm_fence_after();
-            const uint64_t row = tile % tiles_m * 256 + 128 * crank + quad * 32 + lane, n0 = tile / tiles_m * X2_BN;
+            const uint64_t row0 = tile % tiles_m * 256 + 128 * crank + quad * 32, n0 = tile / tiles_m * X2_BN;
 #pragma unroll 1
             for (int c = 0; c < X2_BN / 32; c++) {
                 uint32_t r[32];
                 xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
-                if (row < p.m) xm_store32<TY>(C + row * p.ldc, n0 + c * 32, p.n, p.vec, p.alpha, r);
+                if (row0 < p.m) xm_store32<TY>(C, row0, n0 + c * 32, p, turn, r);
             }
             xm_fence_before();
             __syncwarp();
@@ -659,26 +699,27 @@ static int x1_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
         if (e != cudaSuccess) return status_of(e);
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    // shares of k: as many as keep every SM to one CTA and a share at least four steps long (a cluster's
-    // sum costs about as much as four steps)
+    // shares of k: as many as keep every SM to one CTA and a share at least four steps long, four at most
+    // (100 x 512 x 8192 NVFP4, 4 tiles: 11.7, 10.3, 8.5 and, with eight, 8.9 us; 16 x 1024 x 1024, four
+    // steps: 4.4 us whole, 5.0 in two)
     const uint32_t tiles = (uint32_t)((p.m + XM_BM - 1) / XM_BM * ((p.n + XM_BN - 1) / XM_BN));
     const uint32_t steps = (p.row_bytes + 127) / 128;
-    uint32_t ks = 1;
-    while (ks < 8 && tiles * ks * 2 <= (uint32_t)device_sms() && steps / (ks * 2) >= 4) ks *= 2;
+    uint32_t klog = 0;
+    while (klog < 2 && tiles << (klog + 1) <= (uint32_t)device_sms() && steps >> (klog + 1) >= 4) klog++;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ks;
+    attr[0].val.clusterDim.x = 1u << klog;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(tiles * ks);
-    cfg.blockDim = dim3(XM_THREADS);
+    cfg.gridDim = dim3(tiles << klog);
+    cfg.blockDim = dim3(X1_THREADS);
     cfg.dynamicSmemBytes = Xm<FMT>::kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, mx_mma1_kernel<FMT, TY>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p,
-                           ks, a_rows);
+                           klog, a_rows);
     if (e != cudaSuccess) return status_of(e);
     return last_launch_status();
 }

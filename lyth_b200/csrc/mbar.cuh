@@ -52,6 +52,38 @@ LYTH_D bool mbar_wait(uint32_t bar, uint32_t parity, int *err) {
     return mbar_wait_limited(bar, parity, err, kWaitPolls, kWaitNs);
 }
 
+// The wait of a whole warp in step (all 32 lanes, converged): one try and a vote where the phase is
+// already complete, which is what a pipeline's waits mostly find; the clock is read only once 256
+// tries have failed. Every lane gets the same answer.
+LYTH_D bool mbar_wait_warp(uint32_t bar, uint32_t parity, int *err) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1; i <= kWaitPolls; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (__all_sync(0xFFFFFFFFu, ok)) return true;
+        if ((i & 255u) == 0) {
+            const uint64_t t = global_ns();
+            if (t0 == 0) t0 = t;
+            if (__any_sync(0xFFFFFFFFu, t - t0 > kWaitNs)) break;
+        }
+    }
+    atomicExch(err, 1);
+    return false;
+}
+// One lane of a converged warp; values every lane holds, told to the compiler as uniform.
+LYTH_D bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+LYTH_D uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+
 // Wait until a 64-bit flag in global memory (this GPU's or a peer's, system scope) reaches
 // `target`, polling with acquire loads; on `ns` of global-timer time set *err and return false.
 LYTH_D bool flag_wait_bounded(const uint64_t *flag, uint64_t target, uint64_t ns, int *err) {

@@ -193,7 +193,7 @@ def product_bound(a, b, alpha, k, ty):
     return s * (2 * k + 4) * 2.0 ** -24 + r * (HALF_STEP[ty] + 2.0 ** -23) + (2.0 ** -25 if ty == torch.float16 else 0)
 
 
-MM = [(1, 1, 1), (128, 128, 128), (5, 130, 64), (128, 128, 1024), (200, 136, 192), (257, 300, 1000), (1, 1000, 2048), (300, 515, 4160),
+MM = [(1, 1, 1), (130, 20000, 320), (2500, 1111, 256), (128, 128, 128), (5, 130, 64), (128, 128, 1024), (200, 136, 192), (257, 300, 1000), (1, 1000, 2048), (300, 515, 4160),
       (33, 16, 12288), (1024, 2056, 96)]
 
 
