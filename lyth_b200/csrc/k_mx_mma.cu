@@ -365,9 +365,11 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
 // ---------------------------------------------------------------------------------------------
 // The 2-SM form: a CTA pair computes a 256 x 192 tile with tcgen05.mma.cta_group::2. Each CTA stages
 // its 128 rows of A and 96 of the tile's 192 rows of B, so a 128-byte step moves 28 KiB into an SM for
-// the work that takes the 128 x 128 form 42 KiB: at 4 bits that form is bound by this traffic, not by
-// the tensor cores. 192 columns leave room in tensor memory for two accumulators (2 x 192) beside two
-// sets of scales (2 x 48): the epilogue runs beside the next tile, which 256 columns would not allow.
+// the work that takes the 128 x 128 form 42 KiB: at 4 bits it is this traffic that bounds, 47 bytes a
+// cycle into an SM measured, not the tensor cores. 192 columns leave room in tensor memory for two
+// accumulators (2 x 192) beside two sets of scales. NT = 1: the accumulators take turns, and the
+// epilogue of a tile runs beside the next. NT = 2: a tile of 256 x 384 uses both, a third less traffic
+// for the work, with the epilogue partly exposed; chosen where it leaves fewer rounds (launch rule).
 //
 //   both CTAs, warp 0    producer: its halves of A and B as boxes that complete on the leader's `full`
 //                        barrier; its 128 rows' A scales and the B scales of all 192 columns (the pair's
@@ -382,15 +384,17 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
 // B scale tiles are 128 rows and the tile's 192 start on a multiple of 64: two tiles cover them, and
 // an odd start reads from two tensor-memory columns (64 rows) on.
 constexpr int X2_BN = 192, X2_HALF = X2_BN / 2;
-constexpr int X2_B_BYTES = X2_HALF * 128;
+constexpr int X2_B_BYTES = X2_HALF * 128;      // this CTA's rows of B for one accumulator
 constexpr uint32_t X2_SF_COL = 2 * X2_BN;
 constexpr int X2_THREADS = 320;
 
-template <int FMT>
+template <int FMT, int NT>
 struct X2 {
     static constexpr int kTiles = Xm<FMT>::kTiles;
-    static constexpr int kStageBytes = XM_OP_BYTES + X2_B_BYTES + 3 * kTiles * 512;
-    static constexpr int kSetCols = 12 * kTiles;                     // a step's scales in tensor memory
+    static constexpr int kBTiles = NT + 1;                           // of 128 rows, that hold the tile's columns
+    static constexpr int kSfBytes = (1 + kBTiles) * kTiles * 512;
+    static constexpr int kStageBytes = XM_OP_BYTES + NT * X2_B_BYTES + kSfBytes;
+    static constexpr int kSetCols = 4 * kTiles * (1 + kBTiles);      // a step's scales in tensor memory
     static constexpr int kSets = 128 / kSetCols < 4 ? 128 / kSetCols : 4;
     static constexpr int kTurnBytes = 4 * XM_TURN * 4;               // the epilogue's, at 256 bytes past the ring
     static constexpr int kStages = (227 * 1024 - 1280 - kTurnBytes) / kStageBytes;
@@ -424,16 +428,17 @@ LYTH_D void x2_commit(uint32_t bar) {  // on this barrier in both CTAs
         : "memory");
 }
 
-template <int FMT, int TY>
+template <int FMT, int TY, int NT>
 __global__ void __launch_bounds__(X2_THREADS, 1)
     mx_mma2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                    typename MxElem<TY>::type *C, XmArgs p) {
-    constexpr int T = X2<FMT>::kTiles, S = X2<FMT>::kStages, kSets = X2<FMT>::kSets;
+    using L = X2<FMT, NT>;
+    constexpr int T = L::kTiles, S = L::kStages, kSets = L::kSets, NB = L::kBTiles;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * X2_B_BYTES, *sSB = sSA + S * T * 512;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + S * 2 * T * 512);
+    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * NT * X2_B_BYTES, *sSB = sSA + S * T * 512;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + S * NB * T * 512);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 4 + 4);
     auto full = [&](int s) { return smem_u32(bars + s); };
     auto empty = [&](int s) { return smem_u32(bars + S + s); };
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
 
     const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t crank = blockIdx.x & 1, pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;  // clusters of 2 along x
-    const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + X2_BN - 1) / X2_BN, ntiles = tiles_m * tiles_n;
+    const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + NT * X2_BN - 1) / (NT * X2_BN), ntiles = tiles_m * tiles_n;
     const uint32_t steps = (p.row_bytes + 127) / 128;
 
     if (threadIdx.x == 32) {
@@ -483,17 +488,20 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
         const uint32_t lead = warp_uniform(mapa_shared(full(0), 0));  // the leader's `full` barriers
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
             const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
-            const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * X2_BN);
+            const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * (NT * X2_BN));
             for (uint32_t kb = 0; kb < steps; kb++) {
                 if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
                 const uint32_t lf = lead + 8 * stage;
                 if (elect_one()) {
-                    mbar_expect_tx(sfull(stage), 3 * T * 512);
+                    mbar_expect_tx(sfull(stage), L::kSfBytes);
                     xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
-                    xm_tma3(smem_u32(sSB + stage * 2 * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
-                    mbar_expect_tx_cluster(lf, XM_OP_BYTES + X2_B_BYTES);
+                    xm_tma3(smem_u32(sSB + stage * NB * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
+                    mbar_expect_tx_cluster(lf, XM_OP_BYTES + NT * X2_B_BYTES);
                     x2_tma2(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), m0, lf);
-                    x2_tma2(smem_u32(sB + stage * X2_B_BYTES), &tmB, (int)(kb * 128), n0 + X2_HALF * (int)crank, lf);
+#pragma unroll
+                    for (int h = 0; h < NT; h++)
+                        x2_tma2(smem_u32(sB + (stage * NT + h) * X2_B_BYTES), &tmB, (int)(kb * 128),
+                                n0 + h * X2_BN + X2_HALF * (int)crank, lf);
                 }
                 __syncwarp();
                 if (++stage == S) { stage = 0; phase ^= 1; }
@@ -511,29 +519,34 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
             uint32_t stage = 0, phase = 0, local = 0, set = 0, sphase = 0;
             bool ok = true;
             for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
-                const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
-                if (!xm_wait(tempty(ab), aphase ^ 1)) { ok = false; break; }
-                xm_fence_after();
-                const uint32_t d = tmem_base + ab * X2_BN;
-                const uint32_t shift = ((uint32_t)(tile / tiles_m) & 1) * 2;  // 192 tn is 64 mod 128
+                // one accumulator a tile, in turn; or both
+                const uint32_t ab = NT == 1 ? local & 1 : 0u, aphase = NT == 1 ? (local >> 1) & 1 : local & 1;
+                const uint32_t shift = NT == 1 ? ((uint32_t)(tile / tiles_m) & 1) * 2 : 0u;  // 192 tn is 64 mod 128
                 for (uint32_t kb = 0; kb < steps; kb++) {
                     if (!xm_wait(full(stage), phase) || !xm_wait(sready(set), sphase)) { ok = false; break; }
-                    xm_fence_after();
                     const uint32_t left = p.row_bytes - kb * 128;
                     const int mmas = left < 128 ? (int)(left / 32) : 4;
-                    const uint32_t sfa = tmem_base + X2_SF_COL + set * X2<FMT>::kSetCols, sfb = sfa + 4 * T + shift;
-                    const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES)), b = xm_desc_op(smem_u32(sB + stage * X2_B_BYTES));
-                    if (elect_one()) {
+                    const uint32_t sfa = tmem_base + X2_SF_COL + set * L::kSetCols, sfb = sfa + 4 * T + shift;
+                    const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES));
+                    const uint64_t b = xm_desc_op(smem_u32(sB + stage * NT * X2_B_BYTES));
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            if (j < mmas)
-                                x2_mma<FMT>(d, a + 2 * j, b + 2 * j, xm_idesc<FMT>(X2_BN, 256, j), sfa + 4 * (j * T / 4),
-                                            sfb + 8 * (j * T / 4), (kb | (uint32_t)j) != 0);
+                    for (int h = 0; h < NT; h++) {
+                        if (kb == 0 && !xm_wait(tempty(ab + h), aphase ^ 1)) { ok = false; break; }
+                        xm_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                if (j < mmas)  // columns 192 h on: six words of scales
+                                    x2_mma<FMT>(tmem_base + (ab + h) * X2_BN, a + 2 * j, b + h * (X2_B_BYTES / 16) + 2 * j,
+                                                xm_idesc<FMT>(X2_BN, 256, j), sfa + 4 * (j * T / 4),
+                                                sfb + 4 * NB * (j * T / 4) + 6 * h, (kb | (uint32_t)j) != 0);
+                            }
+                            if (h == NT - 1) x2_commit(empty(stage));
+                            if (kb + 1 == steps) x2_commit(tfull(ab + h));
                         }
-                        x2_commit(empty(stage));
-                        if (kb + 1 == steps) x2_commit(tfull(ab));
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     if (++stage == S) { stage = 0; phase ^= 1; }
                     if (++set == kSets) { set = 0; sphase ^= 1; }
                 }
@@ -564,14 +577,15 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                 }
                 if (!xm_wait(sfull(stage), phase)) { ok = false; break; }
                 xm_fence_after();
-                const uint32_t at = tmem_base + ((quad * 32) << 16) + X2_SF_COL + set * X2<FMT>::kSetCols;
+                const uint32_t at = tmem_base + ((quad * 32) << 16) + X2_SF_COL + set * L::kSetCols;
                 // a tile is 16 bytes a lane: its words of four columns
-                const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * 2 * T * 512 + lane * 16;
+                const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * NB * T * 512 + lane * 16;
 #pragma unroll
                 for (int t = 0; t < T; t++) {
                     x1_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(a + t * 512));
-                    x1_st4(at + 4 * T + 8 * t, *reinterpret_cast<const uint4 *>(b + t * 512));
-                    x1_st4(at + 4 * T + 8 * t + 4, *reinterpret_cast<const uint4 *>(b + (T + t) * 512));
+#pragma unroll
+                    for (int h = 0; h < NB; h++)
+                        x1_st4(at + 4 * T + 4 * NB * t + 4 * h, *reinterpret_cast<const uint4 *>(b + (h * T + t) * 512));
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 xm_fence_before();
@@ -586,20 +600,24 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
         const uint32_t lead_tempty[2] = {mapa_shared(tempty(0), 0), mapa_shared(tempty(1), 0)};
         float *turn = reinterpret_cast<float *>(bars + 32) + quad * XM_TURN;
         uint32_t local = 0;
-        for (uint64_t tile = pair; tile < ntiles; tile += npairs, local++) {
-            const uint32_t ab = local & 1, aphase = (local >> 1) & 1;
-            if (!xm_wait(tfull(ab), aphase)) break;
-            xm_fence_after();
-            const uint64_t row0 = tile % tiles_m * 256 + 128 * crank + quad * 32, n0 = tile / tiles_m * X2_BN;
+        bool ok = true;
+        for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
+            const uint64_t row0 = tile % tiles_m * 256 + 128 * crank + quad * 32, n0 = tile / tiles_m * (NT * X2_BN);
 #pragma unroll 1
-            for (int c = 0; c < X2_BN / 32; c++) {
-                uint32_t r[32];
-                xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
-                if (row0 < p.m) xm_store32<TY>(C, row0, n0 + c * 32, p, turn, r);
+            for (uint32_t h = 0; h < NT; h++) {
+                const uint32_t ab = NT == 1 ? local & 1 : h, aphase = NT == 1 ? (local >> 1) & 1 : local & 1;
+                if (!xm_wait(tfull(ab), aphase)) { ok = false; break; }
+                xm_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < X2_BN / 32; c++) {
+                    uint32_t r[32];
+                    xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
+                    if (row0 < p.m) xm_store32<TY>(C, row0, n0 + h * X2_BN + c * 32, p, turn, r);
+                }
+                xm_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead_tempty[ab]);
             }
-            xm_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(lead_tempty[ab]);
         }
     }
     __syncwarp();
@@ -639,12 +657,13 @@ static bool xm_map_sf(CUtensorMap *map, const void *base, uint64_t words, uint64
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT, int TY>
+template <int FMT, int TY, int NT>
 static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &p, cudaStream_t s) {
-    constexpr int T = X2<FMT>::kTiles;
+    using L = X2<FMT, NT>;
+    constexpr int T = L::kTiles;
     CUtensorMap ta, tb, tsa, tsb;
     if (!xm_map(&ta, a, p.row_bytes, p.m, 128) || !xm_map(&tb, b, p.row_bytes, p.n, X2_HALF) ||
-        !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, 2))
+        !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, L::kBTiles))
         return LYTH_E_UNSUPPORTED;
     static int fit_of[64] = {0};  // pairs resident at once, asked once per device
     int dev = 0;
@@ -657,27 +676,27 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.blockDim = dim3(X2_THREADS);
-    cfg.dynamicSmemBytes = X2<FMT>::kSmem;
+    cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int pairs = device_sms() / 2;
     if (dev < 0 || dev >= 64 || fit_of[dev] == 0) {
-        e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)X2<FMT>::kSmem);
+        e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
         if (e != cudaSuccess) return status_of(e);
         cfg.gridDim = dim3(2u * (unsigned)pairs);
         int fit = 0;
-        if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
+        if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY, NT>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
         cudaGetLastError();
         if (fit < pairs) pairs = fit;
         if (dev >= 0 && dev < 64) fit_of[dev] = pairs;
     } else {
         pairs = fit_of[dev];
     }
-    const uint64_t tiles = (p.m + 255) / 256 * ((p.n + X2_BN - 1) / X2_BN);
+    const uint64_t tiles = (p.m + 255) / 256 * ((p.n + NT * X2_BN - 1) / (NT * X2_BN));
     if ((uint64_t)pairs > tiles) pairs = (int)tiles;
     cfg.gridDim = dim3(2u * (unsigned)pairs);
-    e = cudaLaunchKernelEx(&cfg, mx_mma2_kernel<FMT, TY>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p);
+    e = cudaLaunchKernelEx(&cfg, mx_mma2_kernel<FMT, TY, NT>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p);
     if (e != cudaSuccess) return status_of(e);
     return last_launch_status();
 }
@@ -760,7 +779,16 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     // one tile per SM at most: single SMs, else pairs
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
     if (tiles > (uint64_t)device_sms()) {
-        LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY>(a, b, c, p, s)));
+        // Rounds of all pairs over the tiles: of 192 columns, or of 384, whose round is twice the work in 0.85
+        // (NVFP4; 0.9 of the others) of twice the time. 4096 x 14336 x 4096: 17 rounds against 9, 123 and
+        // 108 us; 4096^3 MXFP4: 5 against 3, 35 and 38 us.
+        const uint64_t pairs = (uint64_t)device_sms() / 2, rows = ((uint64_t)m + 255) / 256;
+        const uint64_t one = (rows * (((uint64_t)n + X2_BN - 1) / X2_BN) + pairs - 1) / pairs;
+        const uint64_t two = (rows * (((uint64_t)n + 2 * X2_BN - 1) / (2 * X2_BN)) + pairs - 1) / pairs;
+        if (20 * one > 2 * two * (fmt == LYTH_MX_NVFP4 ? 17 : 18)) {
+            LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 2>(a, b, c, p, s)));
+        }
+        LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 1>(a, b, c, p, s)));
     }
     LYTH_MX_DISPATCH(fmt, ty, return (x1_launch<FMT, TY>(a, b, c, p, s)));
     return LYTH_E_UNSUPPORTED;
