@@ -27,9 +27,9 @@
 // registers, took 13.2 us for one token through 14336 x 4096 NVFP4 weights: 9.5 us without the loads,
 // 10.6 us without the arithmetic.
 //
-// Range: bf16 x is brought into f16 by one power of two for all of x (its largest finite exponent to
-// 2^14), undone in f32 at the end. Values below 2^-38 of the largest lose bits, which is below the
-// rounding of the f32 sum; every other bf16 value keeps all its bits.
+// Range: bf16 x is brought into f16 by a power of two for each step's columns (128, of E4M3 weights 64
+// neighbouring values of a token; their largest exponent to 2^14) and taken back in f32. Of those values,
+// ones below 2^-32 of the largest lose bits; every other product is exact before the f32 sums.
 #include "mbar.cuh"
 #include "mx.cuh"
 
@@ -125,23 +125,17 @@ LYTH_D uint32_t xv_top(uint4 u) {
     }
     return top;
 }
-// Eight values in f16: f16 as they are, bf16 times a power of two.
-template <int TY>
+// Eight bf16 values times a power of two, in f16.
 LYTH_D uint4 xv_f16(uint4 u, float scale) {
-    if constexpr (TY == LYTH_NARROW_F16) {
-        return u;
-    } else {
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = mx_mul2(mx_unpack2<TY>(w[i]), make_float2(scale, scale));
-            w[i] = mx_pack2<LYTH_NARROW_F16>(f.x, f.y);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; i++) {
+        const float2 f = mx_mul2(mx_unpack2<LYTH_NARROW_BF16>(w[i]), make_float2(scale, scale));
+        w[i] = mx_pack2<LYTH_NARROW_F16>(f.x, f.y);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-LYTH_D void xv_sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(32 * XV_WARPS) : "memory"); }
 LYTH_D bool xv_wait(uint32_t bar, uint32_t parity) { return mbar_wait_warp(bar, parity, &g_xv_error); }
 
 // Where a block is in its walk: batches of groups, chunks of k, groups, segments. All roles take the
@@ -168,11 +162,11 @@ LYTH_D uint32_t xv_row(uint32_t quad, uint32_t j) { return (quad >> 5) * 128 + (
 
 // U steps (it, it + XV_TEAM, ..) of a warp in the stage at `at`, independent of one another until
 // their sums meet in acc: acc[pair][row g, row g + 8] of token t / 2 of the pair. `words`: scale words
-// that the row still has from the stage on. x_off: of step `it` in shared x, bytes.
-template <int FMT, int PAIRS, int U>
-LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_off, uint32_t g, uint32_t t, bool mine,
-                     const uint32_t (&x_at)[PAIRS], uint32_t words, uint4 (&xb)[4],
-                     float (&acc)[PAIRS][2]) {
+// that the row still has from the stage on. x_step: of step `it` in shared x.
+template <int FMT, int TY, int PAIRS, int U>
+LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_step, uint32_t g, uint32_t t, bool mine,
+                     const uint32_t (&x_at)[PAIRS], const float *const (&xs_at)[PAIRS], uint32_t words,
+                     uint4 (&xb)[4], float (&acc)[PAIRS][2]) {
     constexpr int kUnits = FMT == LYTH_MX_FP8 ? 2 : 4, kSub = FMT == LYTH_MX_NVFP4 ? 2 : 1;
     uint4 u0[U], u1[U];
     uint32_t q0[U], q1[U];
@@ -198,7 +192,7 @@ LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_off, uint32_t g,
 #pragma unroll
             for (int pr = 0; pr < PAIRS; pr++) {
                 uint4 &v = xb[(s * PAIRS + pr) % 4];
-                xv_load_x(v, x_at[pr] + x_off + s * (XV_TEAM * 4 * kUnits * 16) + 64 * j, mine);
+                xv_load_x(v, x_at[pr] + (x_step + s * XV_TEAM) * (4 * kUnits * 16) + 64 * j, mine);
                 xv_mma(cc[s][pr][j * kSub / kUnits], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
                 xv_mma(cc[s][pr][j * kSub / kUnits], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
             }
@@ -225,14 +219,29 @@ LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_off, uint32_t g,
             f1[0].x = f1[0].y = mx_scales2<FMT>((q1[s] >> sh) & 0xFFu).x;
         }
 #pragma unroll
-        for (int pr = 0; pr < PAIRS; pr++)
+        for (int pr = 0; pr < PAIRS; pr++) {
+            if constexpr (TY == LYTH_NARROW_BF16) {  // the step's sum, then back from x's f16 range
+                float d0 = 0.0f, d1 = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kSub; k++) {
-                acc[pr][0] = __fmaf_rn(cc[s][pr][k][0], f0[k].x, acc[pr][0]);
-                acc[pr][1] = __fmaf_rn(cc[s][pr][k][2], f1[k].x, acc[pr][1]);
-                acc[pr][0] = __fmaf_rn(cc[s][pr][k][1], f0[k].y, acc[pr][0]);
-                acc[pr][1] = __fmaf_rn(cc[s][pr][k][3], f1[k].y, acc[pr][1]);
+                for (int k = 0; k < kSub; k++) {
+                    d0 = __fmaf_rn(cc[s][pr][k][0], f0[k].x, d0);
+                    d1 = __fmaf_rn(cc[s][pr][k][2], f1[k].x, d1);
+                    d0 = __fmaf_rn(cc[s][pr][k][1], f0[k].y, d0);
+                    d1 = __fmaf_rn(cc[s][pr][k][3], f1[k].y, d1);
+                }
+                const float xs = xs_at[pr][x_step + s * XV_TEAM];
+                acc[pr][0] = __fmaf_rn(d0, xs, acc[pr][0]);
+                acc[pr][1] = __fmaf_rn(d1, xs, acc[pr][1]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSub; k++) {
+                    acc[pr][0] = __fmaf_rn(cc[s][pr][k][0], f0[k].x, acc[pr][0]);
+                    acc[pr][1] = __fmaf_rn(cc[s][pr][k][2], f1[k].x, acc[pr][1]);
+                    acc[pr][0] = __fmaf_rn(cc[s][pr][k][1], f0[k].y, acc[pr][0]);
+                    acc[pr][1] = __fmaf_rn(cc[s][pr][k][3], f1[k].y, acc[pr][1]);
+                }
             }
+        }
     }
 }
 
@@ -244,15 +253,14 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     using T = typename MxElem<TY>::type;
     constexpr int kUnits = FMT == LYTH_MX_FP8 ? 2 : 4;    // 16-byte units of f16 x of a lane per step
     constexpr int kU = PAIRS == 4 ? 1 : 2;                // steps a warp takes at once
-    constexpr uint32_t kStepX = 4 * kUnits * 16;          // bytes of x of a step and token
     constexpr int kTokens = 2 * PAIRS;
     extern __shared__ __align__(128) uint8_t sm[];        // ring, x, partial sums
     __shared__ uint64_t bars[2 * 4 + 1];
-    __shared__ uint32_t s_max[XV_WARPS];
     const uint32_t warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t xunits = p.xsteps * 4 * kUnits;        // 16-byte units of x per token
     uint4 *sx = reinterpret_cast<uint4 *>(sm + p.stages * Xv<FMT>::kStage);
-    float *s_part = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // [group][warp][token][row]
+    float *s_scale = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // of bf16 x: [token][step]
+    float *s_part = s_scale + (TY == LYTH_NARROW_BF16 ? p.m * p.xsteps : 0);  // [group][warp][token][row]
     auto full = [&](uint32_t s) { return smem_u32(bars + s); };
     auto empty = [&](uint32_t s) { return smem_u32(bars + 4 + s); };
     const uint32_t xbar = smem_u32(bars + 8);             // the consumers' meeting point
@@ -326,39 +334,10 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
 #pragma unroll
         for (int pr = 0; pr < PAIRS; pr++)
             x_at[pr] = smem_u32(sx + min(2u * pr + (g >> 2), p.m - 1) * (xunits + 4) + t);
+        const float *xs_at[PAIRS];  // of this lane's columns' token
+#pragma unroll
+        for (int pr = 0; pr < PAIRS; pr++) xs_at[pr] = s_scale + min(2u * pr + (t >> 1), p.m - 1) * p.xsteps;
         const T *x = static_cast<const T *>(p.x);
-        float scale = 1.0f;
-        // Units of x, token after token, four of a thread's loads in flight; `per` units of a token from
-        // unit `first` on.
-        auto each = [&](uint32_t first, uint32_t per, auto &&use) {
-#pragma unroll 1
-            for (uint32_t i0 = threadIdx.x; i0 < p.m * per; i0 += 4 * 32 * XV_WARPS) {
-                uint4 v[4];
-                uint32_t tok[4], u[4];
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const uint32_t i = i0 + h * 32 * XV_WARPS;
-                    tok[h] = p.m == 1 ? 0u : i / per;
-                    u[h] = i - tok[h] * per;
-                    if (i < p.m * per) v[h] = xv_load8<TY>(x + tok[h] * p.ldx, 8 * (first + u[h]), p.cols, p.vec);
-                }
-#pragma unroll
-                for (int h = 0; h < 4; h++)
-                    if (i0 + h * 32 * XV_WARPS < p.m * per) use(tok[h], u[h], v[h]);
-            }
-        };
-        if constexpr (TY == LYTH_NARROW_BF16) {
-            uint32_t top = 0;
-            each(0, (p.cols + 7) / 8, [&](uint32_t, uint32_t, uint4 v) { top = max(top, xv_top(v)); });
-            top = __reduce_max_sync(0xFFFFFFFFu, top);
-            if (lane == 0) s_max[warp] = top;
-            xv_sync_consumers();
-            top = __reduce_max_sync(0xFFFFFFFFu, lane < XV_WARPS ? s_max[lane] : 0u);
-            // 2^(14 - e), e the largest exponent; it and its inverse kept within normal f32 numbers
-            const int sh = min(14 - ((int)top - 127), 126);
-            scale = __uint_as_float((uint32_t)(sh + 127) << 23);
-        }
-        const float unscale = __uint_as_float((254u << 23) - __float_as_uint(scale));
         uint32_t stage = 0, phase = 0, turn = 1;
         bool ok = true, staged = false;
         uint32_t xphase = 0;
@@ -376,10 +355,38 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                     // (a bounded meeting: a warp that gave up a wait has left)
                     if (staged && !(ok = meet())) break;
                     const uint32_t first = c0 * XV_STEPS * 4 * kUnits;
-                    each(first, xunits, [&](uint32_t tok, uint32_t u, uint4 v) {
-                        const uint32_t at = u / (4 * kUnits) * (4 * kUnits) + u % kUnits * 4 + u / kUnits % 4;
-                        sx[tok * (xunits + 4) + at] = xv_f16<TY>(v, scale);
-                    });
+                    // Units of x, token after token, four of a thread's loads in flight; whole warps, since a
+                    // step's units (16, of E4M3 codes 8) lie in neighbouring lanes and share a power of two.
+                    const uint32_t all = p.m * xunits;
+#pragma unroll 1
+                    for (uint32_t i0 = threadIdx.x; i0 - lane < all; i0 += 4 * 32 * XV_WARPS) {
+                        uint4 v[4];
+                        uint32_t tok[4], u[4];
+#pragma unroll
+                        for (int h = 0; h < 4; h++) {
+                            const uint32_t i = i0 + h * 32 * XV_WARPS;
+                            tok[h] = p.m == 1 ? 0u : i / xunits;
+                            u[h] = i - tok[h] * xunits;
+                            v[h] = make_uint4(0, 0, 0, 0);
+                            if (i < all) v[h] = xv_load8<TY>(x + tok[h] * p.ldx, 8 * (first + u[h]), p.cols, p.vec);
+                        }
+#pragma unroll
+                        for (int h = 0; h < 4; h++) {
+                            const bool in = i0 + h * 32 * XV_WARPS < all;
+                            const uint32_t owner = u[h] / kUnits;  // step and quad lane
+                            if constexpr (TY == LYTH_NARROW_BF16) {
+                                uint32_t top = xv_top(v[h]);
+#pragma unroll
+                                for (int o = 1; o < 4 * kUnits; o *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                                // 2^(14 - e), e the largest exponent; it and its inverse are normal f32 numbers
+                                const int sh = min(14 - ((int)top - 127), 126);
+                                v[h] = xv_f16(v[h], __uint_as_float((uint32_t)(127 + sh) << 23));
+                                if (in && u[h] % (4 * kUnits) == 0)
+                                    s_scale[tok[h] * p.xsteps + owner / 4] = __uint_as_float((uint32_t)(127 - sh) << 23);
+                            }
+                            if (in) sx[tok[h] * (xunits + 4) + owner / 4 * (4 * kUnits) + u[h] % kUnits * 4 + owner % 4] = v[h];
+                        }
+                    }
                     if (!(ok = meet())) break;
                     staged = true;
                 }
@@ -395,13 +402,13 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                         if (!xv_wait(full(stage), phase)) { ok = false; break; }
                         const uint8_t *at = sm + stage * Xv<FMT>::kStage;
                         const uint32_t steps = (min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG) + 63) / 64;
-                        const uint32_t words = p.words - seg * Xv<FMT>::kWords, x_base = (seg - c0) * XV_STEPS * kStepX;
+                        const uint32_t words = p.words - seg * Xv<FMT>::kWords, x_base = (seg - c0) * XV_STEPS;
                         uint32_t it = warp % XV_TEAM;
                         for (; it + (kU - 1) * XV_TEAM < steps; it += kU * XV_TEAM)
-                            xv_steps<FMT, PAIRS, kU>(at, it, x_base + it * kStepX, g, t, mine, x_at, words, xb, acc);
+                            xv_steps<FMT, TY, PAIRS, kU>(at, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
                         if constexpr (kU > 1)
                             for (; it < steps; it += XV_TEAM)
-                                xv_steps<FMT, PAIRS, 1>(at, it, x_base + it * kStepX, g, t, mine, x_at, words, xb, acc);
+                                xv_steps<FMT, TY, PAIRS, 1>(at, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
                         __syncwarp();
                         if (lane == 0) mbar_arrive(empty(stage));
                         if (++stage == p.stages) { stage = 0; phase ^= 1; }
@@ -430,7 +437,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                 for (int k = 0; k < XV_WARPS; k++) v = __fadd_rn(v, part[k * kTokens * 16]);
                 if (quad < w.hi && row <= w.last)
                     static_cast<T *>(p.y)[tok * p.ldy + w.tile0 * 128 + row] =
-                        MxElem<TY>::round(__fmul_rn(p.alpha, __fmul_rn(v, unscale)));
+                        MxElem<TY>::round(__fmul_rn(p.alpha, v));
             }
             if (w.hi - w.lo == 4 * kXvBatch<PAIRS> && !(ok = meet())) break;  // before the next batch's sums
         }
@@ -447,7 +454,7 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
     // least a segment: 8 tokens x 2048 E2M1 bytes are 64 KiB).
     const uint32_t groups = (p.quads_each + (p.quads_more ? 1 : 0) + 3) / 4;
     const size_t sums = (size_t)(groups < (uint32_t)kXvBatch<PAIRS> ? groups : kXvBatch<PAIRS>) * XV_WARPS * 2 * PAIRS * 16 * sizeof(float);
-    const size_t step_x = (size_t)p.m * (FMT == LYTH_MX_FP8 ? 8 : 16) * 16;
+    const size_t step_x = (size_t)p.m * ((FMT == LYTH_MX_FP8 ? 8 : 16) * 16 + (TY == LYTH_NARROW_BF16 ? 4 : 0));
     const uint32_t steps = (p.row_bytes + 63) / 64;
     const size_t room = 226 * 1024 - sums - p.m * 64;
     p.stages = 4;

@@ -40,17 +40,14 @@ inline uint64_t mx_code_bytes(int fmt, uint64_t k) { return fmt == LYTH_MX_FP8 ?
 template <int TY> struct MxElem;
 template <> struct MxElem<0> {
     using type = float;
-    LYTH_D static float load(const float *p) { return *p; }
     LYTH_D static float round(float v) { return v; }
 };
 template <> struct MxElem<LYTH_NARROW_F16> {
     using type = __half;
-    LYTH_D static float load(const __half *p) { return __half2float(*p); }
     LYTH_D static __half round(float v) { return __float2half_rn(v); }
 };
 template <> struct MxElem<LYTH_NARROW_BF16> {
     using type = __nv_bfloat16;
-    LYTH_D static float load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
     LYTH_D static __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
 };
 inline bool mx_ty_known(int ty) { return ty == 0 || ty == LYTH_NARROW_F16 || ty == LYTH_NARROW_BF16; }
@@ -76,28 +73,6 @@ LYTH_D float2 mx_unpack2(uint32_t u) {
     }
 }
 
-// Eight consecutive values of a row, `col` a multiple of 8, zero behind `cols`. `vec`: every row
-// starts on 16 bytes.
-template <int TY>
-LYTH_D void mx_load8(const typename MxElem<TY>::type *row, uint32_t col, uint32_t cols, bool vec, float (&v)[8]) {
-    if (vec && col + 8 <= cols) {
-        if constexpr (TY == 0) {
-            const float4 a = *reinterpret_cast<const float4 *>(row + col);
-            const float4 b = *reinterpret_cast<const float4 *>(row + col + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4 *>(row + col);
-            const float2 a = mx_unpack2<TY>(u.x), b = mx_unpack2<TY>(u.y), c = mx_unpack2<TY>(u.z),
-                         d = mx_unpack2<TY>(u.w);
-            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-            v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = col + i < cols ? MxElem<TY>::load(row + col + i) : 0.0f;
-    }
-}
 // ---- rows of the unquantised side, 16 values ("a chunk") at a time.
 // A chunk is 8 words of a 16-bit type, 16 of f32. VEC: every row starts on 32 bytes and is whole
 // chunks, which move in 256-bit accesses (two 128-bit stores 32 bytes apart per lane write every

@@ -187,10 +187,12 @@ def test_rmsnorm_in_place_and_poisoned_row(cuda):
 def product_bound(a, b, alpha, k, ty):
     """f32 accumulation of k exact products in any order, alpha's and the output's rounding. The
     tensor cores align a step's products and may cut instead of round (up to 2^-23 of the largest
-    partial sum each step): 2 k 2^-24 of the sum of magnitudes covers a chain of k of either."""
+    partial sum each step): 2 k 2^-24 of the sum of magnitudes covers a chain of k of either. Results
+    below a type's smallest normal number are off by half its smallest step at most: f16 2^-25, bf16
+    2^-134 (its step there is 2^-133), f32 2^-150 for each of k sums."""
     s = np.abs(a) @ np.abs(b).T * abs(alpha)
     r = np.abs(a @ b.T) * abs(alpha)
-    return s * (2 * k + 4) * 2.0 ** -24 + r * (HALF_STEP[ty] + 2.0 ** -23) + (2.0 ** -25 if ty == torch.float16 else 0)
+    return s * (2 * k + 4) * 2.0 ** -24 + r * (HALF_STEP[ty] + 2.0 ** -23) + {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 0.0}[ty] + k * 2.0 ** -150
 
 
 MM = [(1, 1, 1), (130, 20000, 320), (2500, 1111, 256), (128, 128, 128), (5, 130, 64), (128, 128, 1024), (200, 136, 192), (257, 300, 1000), (1, 1000, 2048), (300, 515, 4160),
@@ -231,3 +233,239 @@ def test_gemv(cuda, fmt, ty, m, n, cols):
     want = 0.5 * (vx @ vw[:, :cols].T)
     assert (np.abs(wide(y)[:, :n] - want) <= product_bound(vx, vw[:, :cols], 0.5, cols, ty)).all()
     assert bool((y[:, n:] == 5).all())
+
+
+# ------------------------------------------------------------------ values that are not numbers, and extremes
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n", [(40, 70), (300, 20000)])  # single SMs and CTA pairs
+def test_matmul_bad_and_zero_blocks_stay_in_their_rows(cuda, fmt, m, n):
+    rng = np.random.default_rng(4)
+    k = 512
+    a, sa, va = mx.random_operand(fmt, m, k, rng, 1)
+    b, sb, vb = mx.random_operand(fmt, n, k, rng, 1)
+    where = mx.scale_at(max(m, n), k // mx.BLOCK[fmt])
+    bad, zero = (0x7F if fmt == lb.MX_NVFP4 else 0xFF), 0
+    sa[where[5, 3]] = bad          # one NaN scale: row 5 of the product, and only it
+    sb[where[11, 0]] = bad         # column 11
+    sa[where[7, :]] = zero         # a row of the smallest scales (NVFP4: of zeros)
+    size = {lb.MX_NVFP4: 0.0}.get(fmt, 2.0 ** -127)
+    va[7] = va[7] * 0 + mx.values(fmt, mx.unpack(fmt, a[7:8]), np.zeros((1, k // mx.BLOCK[fmt]), np.int64))[0]
+    assert np.abs(va[7]).max() <= 448 * size
+    dev = [torch.from_numpy(t).to(cuda) for t in (a, sa, b, sb)]
+    c = torch.empty(m, n, device=cuda)
+    lb.matmul_mx(fmt, *dev, c)
+    got = wide(c)
+    nan = np.zeros((m, n), bool)
+    nan[5, :] = nan[:, 11] = True
+    assert np.array_equal(np.isnan(got), nan)
+    want = va @ vb.T
+    ok = ~nan
+    assert (np.abs(got - want)[ok] <= (product_bound(va, vb, 1.0, k, torch.float32) + 2.0 ** -126)[ok]).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ty", TYPES[1:])
+def test_gemv_tokens_do_not_touch_one_another(cuda, fmt, ty):
+    # an infinity, a NaN, a huge, a tiny, a zero and a subnormal token beside ordinary ones
+    m, n, k = 8, 200, 700
+    rng = np.random.default_rng(6)
+    w, sw, vw = mx.random_operand(fmt, n, k, rng, 2)
+    x = torch.from_numpy(rng.standard_normal((m, k)).astype(np.float32))
+    big, tiny = (1e30, 1e-30) if ty == torch.bfloat16 else (60.0, 1e-4)
+    x[1] *= big
+    x[2] *= tiny
+    x[3] = 0
+    x[4, 333] = float("inf")
+    x[5, 17] = float("nan")
+    x[6] *= 1e-39 if ty == torch.bfloat16 else 1e-7
+    x = x.to(ty)
+    vx = x.double().numpy()
+    args = torch.from_numpy(w).to(cuda), torch.from_numpy(sw).to(cuda)
+    y = torch.empty(m, n, dtype=ty, device=cuda)
+    lb.gemv_mx(fmt, x.to(cuda), *args, y)
+    got = wide(y)
+    with np.errstate(invalid="ignore", over="ignore"):
+        want = vx @ vw[:, :k].T
+    assert np.array_equal(np.isnan(got[4:6]), np.isnan(want[4:6]))
+    fin = np.isfinite(want)
+    fin[4:6] = False
+    bound = product_bound(np.where(np.isfinite(vx), vx, 0), vw[:, :k], 1.0, k, ty)
+    top = torch.finfo(ty).max
+    inside = fin & (np.abs(want) < top * 0.99)
+    assert inside[[0, 2, 3, 6, 7]].all()
+    with np.errstate(invalid="ignore"):
+        off = np.abs(got - want)
+    assert (off[inside] <= bound[inside]).all(), np.argwhere(inside & ~(off <= bound))[:5]
+    assert (got[3] == 0).all()
+    inf = ~np.isnan(want[4]) & np.isinf(want[4])
+    assert np.array_equal(got[4][inf], want[4][inf])
+    # each alone gives the same bits
+    for i in (0, 1, 2, 7):
+        one = torch.empty(1, n, dtype=ty, device=cuda)
+        lb.gemv_mx(fmt, x[i:i + 1].to(cuda), *args, one)
+        assert torch.equal(one[0].view(torch.int16), y[i].view(torch.int16)), i
+
+
+def test_gemv_wide_range_within_a_token(cuda):
+    # bf16 columns 2^20 apart, in one block and across blocks: the small ones still count
+    rng = np.random.default_rng(7)
+    n, k = 64, 1024
+    w, sw, vw = mx.random_operand(lb.MX_FP4, n, k, rng, 0)
+    x = torch.from_numpy(rng.standard_normal((1, k)).astype(np.float32))
+    x[0, ::7] *= 2.0 ** 20
+    x[0, 512:] *= 2.0 ** -90
+    x = x.bfloat16()
+    vx = x.double().numpy()
+    y = torch.empty(1, n, dtype=torch.bfloat16, device=cuda)
+    lb.gemv_mx(lb.MX_FP4, x.to(cuda), torch.from_numpy(w).to(cuda), torch.from_numpy(sw).to(cuda), y)
+    assert (np.abs(wide(y) - vx @ vw.T) <= product_bound(vx, vw, 1.0, k, torch.bfloat16)).all()
+    # only the far half of x: its own range
+    x2 = torch.zeros_like(x)
+    x2[0, 512:] = x[0, 512:]
+    v2 = x2.double().numpy()
+    lb.gemv_mx(lb.MX_FP4, x2.to(cuda), torch.from_numpy(w).to(cuda), torch.from_numpy(sw).to(cuda), y)
+    assert (np.abs(wide(y) - v2 @ vw.T) <= product_bound(v2, vw, 1.0, k, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_gemv_strided_and_unaligned_x(cuda, fmt):
+    rng = np.random.default_rng(12)
+    m, n, k = 3, 130, 1001
+    w, sw, vw = mx.random_operand(fmt, n, k, rng, 2)
+    full = torch.from_numpy(rng.standard_normal((m, k + 9)).astype(np.float32)).bfloat16().to(cuda)
+    for off in (0, 1, 8):
+        x = full[:, off:off + k]
+        y = torch.full((m, n + 1), 2.0, dtype=torch.bfloat16, device=cuda)
+        lb.gemv_mx(fmt, x, torch.from_numpy(w).to(cuda), torch.from_numpy(sw).to(cuda), y[:, 1:])
+        vx = wide(x)
+        assert (np.abs(wide(y)[:, 1:] - vx @ vw[:, :k].T) <= product_bound(vx, vw[:, :k], 1.0, k, torch.bfloat16)).all()
+        assert bool((y[:, 0] == 2).all())
+
+
+# ------------------------------------------------------------------ together, and the ways they are called
+def block_ref(fmt, x, r, w_norm, weights, eps):
+    """Norm, quantised; the product with quantised weights; 64 bits throughout but for the formats."""
+    h, y = norm_ref(x, r, w_norm, eps)
+    return h, mx.values(fmt, *mx.quantize(fmt, y)) @ weights.T
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows", [1, 37, 200])
+def test_norm_then_projection(cuda, fmt, rows):
+    # the block as it is used: residual + norm + quantise, then the projection's product on the codes, or
+    # for a few rows on the unquantised activations
+    k, n = 1024, 640
+    rng = np.random.default_rng(30 + rows)
+    gen = torch.Generator().manual_seed(rows)
+    x, r = (torch.randn(rows, k, generator=gen).bfloat16().to(cuda) for _ in range(2))
+    wn = (1 + 0.1 * torch.randn(k, generator=gen)).bfloat16().to(cuda)
+    wf = torch.from_numpy((rng.standard_normal((n, k)) / 32).astype(np.float32)).bfloat16().to(cuda)
+    wq = lb.mx_empty(fmt, n, k, cuda)
+    lb.quantize_mx(fmt, wf, *wq)
+    vw = mx.values(fmt, *mx.quantize(fmt, wide(wf)))
+    aq = lb.mx_empty(fmt, rows, k, cuda)
+    h, c = torch.empty_like(x), torch.empty(rows, n, device=cuda)
+    lb.rmsnorm_mx(fmt, x, wn, *aq, residual=r, residual_out=h, eps=1e-5)
+    lb.matmul_mx(fmt, *aq, *wq, c)
+    _, want = block_ref(fmt, wide(x), wide(r), wide(wn), vw, 1e-5)
+    # the product itself, on the codes the norm really made
+    got_a = torch.empty(rows, k, device=cuda)
+    lb.dequantize_mx(fmt, *aq, got_a)
+    exact = wide(got_a) @ vw.T
+    assert (np.abs(wide(c) - exact) <= product_bound(wide(got_a), vw, 1.0, k, torch.float32)).all()
+    # and end to end: codes at a border may differ by a step (at most 1e-2 of them, test_rmsnorm), each
+    # by half its value at most, so the norm of the difference is at most 0.1 * 0.5 of the whole
+    assert np.linalg.norm(wide(c) - want) <= 0.05 * np.linalg.norm(want)
+    if rows <= lb.GEMV_MX_MAX_M:
+        a16, y = got_a.bfloat16(), torch.empty(rows, n, dtype=torch.bfloat16, device=cuda)
+        lb.gemv_mx(fmt, a16, *wq, y)
+        v16 = wide(a16)
+        assert (np.abs(wide(y) - v16 @ vw.T) <= product_bound(v16, vw, 1.0, k, torch.bfloat16)).all()
+
+
+def all_calls(fmt, s):
+    lb.rmsnorm_mx(fmt, s["x"], s["wn"], *s["a"], residual=s["r"], residual_out=s["h"])
+    lb.matmul_mx(fmt, *s["a"], *s["w"], s["c"])
+    lb.quantize_mx(fmt, s["x"], *s["q"])
+    lb.dequantize_mx(fmt, *s["q"], s["d"])
+    lb.gemv_mx(fmt, s["d"], *s["w"], s["y"])
+
+
+OUTPUTS = ["h", "c", "d", "y"]
+
+
+def state(fmt, cuda, seed, rows=5, k=768, n=400):
+    gen = torch.Generator().manual_seed(seed)
+    s = {"x": torch.randn(rows, k, generator=gen).bfloat16().to(cuda), "r": torch.randn(rows, k, generator=gen).bfloat16().to(cuda),
+         "wn": torch.ones(k, dtype=torch.bfloat16, device=cuda), "a": lb.mx_empty(fmt, rows, k, cuda), "q": lb.mx_empty(fmt, rows, k, cuda),
+         "w": lb.mx_empty(fmt, n, k, cuda), "h": torch.empty(rows, k, dtype=torch.bfloat16, device=cuda),
+         "d": torch.empty(rows, k, dtype=torch.bfloat16, device=cuda), "c": torch.empty(rows, n, device=cuda),
+         "y": torch.empty(rows, n, dtype=torch.bfloat16, device=cuda)}
+    lb.quantize_mx(fmt, torch.randn(n, k, generator=gen).to(cuda), *s["w"])
+    return s
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_captured_and_replayed_on_new_inputs(cuda, fmt):
+    s, t = state(fmt, cuda, 1), state(fmt, cuda, 2)
+    all_calls(fmt, t)
+    want = {o: t[o].clone() for o in OUTPUTS}
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        all_calls(fmt, s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            all_calls(fmt, s)
+    torch.cuda.synchronize()
+    for name in ("x", "r"):
+        s[name].copy_(t[name])
+    for a, b in zip(s["w"], t["w"]):
+        a.copy_(b)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for o in OUTPUTS:
+        assert torch.equal(s[o], want[o]), o
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_two_streams_and_repeats_give_the_same_bits(cuda, fmt):
+    states = [state(fmt, cuda, i) for i in (3, 4)]
+    want = []
+    for s in states:
+        all_calls(fmt, s)
+        want.append({o: s[o].clone() for o in OUTPUTS})
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for s, st in zip(states, streams):
+            with torch.cuda.stream(st):
+                all_calls(fmt, s)
+    for s, st, w in zip(states, streams, want):
+        st.synchronize()
+        for o in OUTPUTS:
+            assert torch.equal(s[o], w[o]), o
+    # an explicit stream, as an object and as its handle
+    s = states[0]
+    s["c"].zero_()
+    torch.cuda.synchronize()
+    lb.matmul_mx(fmt, *s["a"], *s["w"], s["c"], stream=streams[0])
+    streams[0].synchronize()
+    assert torch.equal(s["c"], want[0]["c"])
+    s["c"].zero_()
+    torch.cuda.synchronize()
+    lb.matmul_mx(fmt, *s["a"], *s["w"], s["c"], stream=streams[1].cuda_stream)
+    streams[1].synchronize()
+    assert torch.equal(s["c"], want[0]["c"])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_no_rows_no_columns_of_the_product(cuda, fmt):
+    w = state(fmt, cuda, 9)["w"]
+    for m in (0,):
+        lb.quantize_mx(fmt, torch.empty(m, 768, device=cuda), *lb.mx_empty(fmt, m, 768, cuda))
+        lb.matmul_mx(fmt, *lb.mx_empty(fmt, m, 768, cuda), *w, torch.empty(m, 400, device=cuda))
+        lb.gemv_mx(fmt, torch.empty(m, 768, dtype=torch.float16, device=cuda), *w, torch.empty(m, 400, dtype=torch.float16, device=cuda))
+    lb.matmul_mx(fmt, *w, *lb.mx_empty(fmt, 0, 768, cuda), torch.empty(400, 0, device=cuda))
+    torch.cuda.synchronize()
