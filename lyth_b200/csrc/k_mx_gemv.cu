@@ -39,23 +39,12 @@ __device__ int g_xv_error = 0;
 
 constexpr int XV_WARPS = 16;                        // consumers
 constexpr int XV_TEAM = XV_WARPS / 2;               // a team takes every other stage
+constexpr uint32_t XV_STAGES = 4;                   // of the ring: even, since a team owns every other one
 constexpr int XV_PRODUCERS = 4;                     // warps, one per quad of a group
 constexpr int XV_THREADS = 32 * (XV_WARPS + XV_PRODUCERS);
-constexpr int XV_SEG = 2048;                        // bytes of a row in a stage
-constexpr int XV_ROW = XV_SEG + 64;                 // their pitch: eight rows read at once hit all banks
-constexpr int XV_STEPS = XV_SEG / 64;               // steps in a whole stage
-constexpr int XV_W_BYTES = 16 * XV_ROW;
-
 // Groups whose partial sums are kept before they are added up: all of a block's, up to this many.
 template <int PAIRS>
 constexpr int kXvBatch = PAIRS == 4 ? 4 : 8;
-
-// Scale words of a row in a stage: one for 64 (E4M3: 128) bytes of MX codes, two for 64 of NVFP4.
-template <int FMT>
-struct Xv {
-    static constexpr int kWords = FMT == LYTH_MX_FP8 ? XV_STEPS / 2 : FMT == LYTH_MX_FP4 ? XV_STEPS : 2 * XV_STEPS;
-    static constexpr int kStage = XV_W_BYTES + kWords * 64;  // a quad's four words are 16 bytes
-};
 
 struct XvArgs {
     const void *x;
@@ -65,9 +54,9 @@ struct XvArgs {
     uint32_t m, n, cols;
     uint32_t quads_each, quads_more;  // quads of a block; blocks that have one more
     uint32_t row_bytes, words;        // bytes of a row of codes; scale words along k
-    uint32_t segs;                    // stages along k
+    uint32_t seg, segs;               // bytes of a row in a stage; stages along k
+    uint32_t seg_words, stage_bytes;  // scale words of a row in a stage; 16 rows (pitch seg + 64) and the words
     uint32_t chunk, xsteps;           // segments, and steps, whose x is in shared memory at once
-    uint32_t stages;                  // of the ring
     float alpha;
     bool vec;                         // rows of x start on 16 bytes
 };
@@ -164,7 +153,7 @@ LYTH_D uint32_t xv_row(uint32_t quad, uint32_t j) { return (quad >> 5) * 128 + (
 // their sums meet in acc: acc[pair][row g, row g + 8] of token t / 2 of the pair. `words`: scale words
 // that the row still has from the stage on. x_step: of step `it` in shared x.
 template <int FMT, int TY, int PAIRS, int U>
-LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_step, uint32_t g, uint32_t t, bool mine,
+LYTH_D void xv_steps(const uint8_t *at, uint32_t pitch, uint32_t it, uint32_t x_step, uint32_t g, uint32_t t, bool mine,
                      const uint32_t (&x_at)[PAIRS], const float *const (&xs_at)[PAIRS], uint32_t words,
                      uint4 (&xb)[4], float (&acc)[PAIRS][2]) {
     constexpr int kUnits = FMT == LYTH_MX_FP8 ? 2 : 4, kSub = FMT == LYTH_MX_NVFP4 ? 2 : 1;
@@ -174,12 +163,12 @@ LYTH_D void xv_steps(const uint8_t *at, uint32_t it, uint32_t x_step, uint32_t g
 #pragma unroll
     for (int s = 0; s < U; s++) {
         const uint32_t i = it + s * XV_TEAM;
-        u0[s] = *reinterpret_cast<const uint4 *>(at + g * XV_ROW + i * 64 + t * 16);
-        u1[s] = *reinterpret_cast<const uint4 *>(at + (g + 8) * XV_ROW + i * 64 + t * 16);
+        u0[s] = *reinterpret_cast<const uint4 *>(at + g * pitch + i * 64 + t * 16);
+        u1[s] = *reinterpret_cast<const uint4 *>(at + (g + 8) * pitch + i * 64 + t * 16);
         // the scale word that holds this lane's two columns' blocks
         const uint32_t word = FMT == LYTH_MX_FP8 ? i >> 1 : FMT == LYTH_MX_FP4 ? i : 2 * i + (t & 1);
-        q0[s] = *reinterpret_cast<const uint32_t *>(at + XV_W_BYTES + word * 64 + g * 4);
-        q1[s] = *reinterpret_cast<const uint32_t *>(at + XV_W_BYTES + word * 64 + g * 4 + 32);
+        q0[s] = *reinterpret_cast<const uint32_t *>(at + 16 * pitch + word * 64 + g * 4);
+        q1[s] = *reinterpret_cast<const uint32_t *>(at + 16 * pitch + word * 64 + g * 4 + 32);
         if (FMT == LYTH_MX_NVFP4 && word >= words) q0[s] = q1[s] = 0;  // a row may end in half a step
     }
 #pragma unroll
@@ -255,17 +244,18 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     constexpr int kU = PAIRS == 4 ? 1 : 2;                // steps a warp takes at once
     constexpr int kTokens = 2 * PAIRS;
     extern __shared__ __align__(128) uint8_t sm[];        // ring, x, partial sums
-    __shared__ uint64_t bars[2 * 4 + 1];
+    __shared__ uint64_t bars[2 * XV_STAGES + 1];
     const uint32_t warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t xunits = p.xsteps * 4 * kUnits;        // 16-byte units of x per token
-    uint4 *sx = reinterpret_cast<uint4 *>(sm + p.stages * Xv<FMT>::kStage);
+    const uint32_t pitch = p.seg + 64;                    // of rows in a stage: eight read at once hit all banks
+    uint4 *sx = reinterpret_cast<uint4 *>(sm + XV_STAGES * p.stage_bytes);
     float *s_scale = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // of bf16 x: [token][step]
     float *s_part = s_scale + (TY == LYTH_NARROW_BF16 ? p.m * p.xsteps : 0);  // [group][warp][token][row]
     auto full = [&](uint32_t s) { return smem_u32(bars + s); };
-    auto empty = [&](uint32_t s) { return smem_u32(bars + 4 + s); };
-    const uint32_t xbar = smem_u32(bars + 8);             // the consumers' meeting point
+    auto empty = [&](uint32_t s) { return smem_u32(bars + XV_STAGES + s); };
+    const uint32_t xbar = smem_u32(bars + 2 * XV_STAGES); // the consumers' meeting point
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < p.stages; s++) {
+        for (uint32_t s = 0; s < XV_STAGES; s++) {
             mbar_init(full(s), 33 * XV_PRODUCERS);  // the producers' lanes (scales) and counts of bytes (rows)
             mbar_init(empty(s), XV_TEAM);
         }
@@ -274,7 +264,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     }
     __syncthreads();
 
-    if (warp >= XV_WARPS && warp < XV_WARPS + XV_PRODUCERS) {  // ------------------------------------------------------------- producer
+    if (warp >= XV_WARPS) {  // ------------------------------------------------------------------ producers
         uint32_t stage = 0, phase = 0;
         bool ok = true;
         XvWalk w;
@@ -291,25 +281,25 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                     const uint8_t *ssrc = s_base + (uint64_t)(quad >> 5) * p.words * 512 + (quad & 31) * 16;
                     for (uint32_t seg = c0; seg < c1; seg++) {
                         if (!xv_wait(empty(stage), phase ^ 1)) { ok = false; break; }
-                        const uint32_t bytes = min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG);
-                        const uint32_t at = smem_u32(sm) + stage * Xv<FMT>::kStage;
+                        const uint32_t bytes = min(p.row_bytes - seg * p.seg, p.seg);
+                        const uint32_t at = smem_u32(sm) + stage * p.stage_bytes;
                         if (elect_one()) {
                             mbar_expect_tx(full(stage), rows * bytes);
 #pragma unroll
                             for (uint32_t j = 0; j < 4; j++)
                                 if (j < rows)
-                                    bulk_load(at + (pw * 4 + j) * XV_ROW, src + seg * XV_SEG + (uint64_t)j * 32 * p.row_bytes, bytes,
+                                    bulk_load(at + (pw * 4 + j) * pitch, src + seg * p.seg + (uint64_t)j * 32 * p.row_bytes, bytes,
                                               full(stage));
                         }
                         __syncwarp();
-                        const uint32_t w0 = seg * Xv<FMT>::kWords, nw = min(p.words - w0, (uint32_t)Xv<FMT>::kWords);
+                        const uint32_t w0 = seg * p.seg_words, nw = min(p.words - w0, p.seg_words);
                         if (has)
                             for (uint32_t i = lane; i < nw; i += 32)
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + XV_W_BYTES + i * 64 + pw * 16),
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + 16 * pitch + i * 64 + pw * 16),
                                              "l"(ssrc + (uint64_t)(w0 + i) * 512)
                                              : "memory");
                         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(stage)) : "memory");
-                        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                        if (++stage == XV_STAGES) { stage = 0; phase ^= 1; }
                     }
                 }
             }
@@ -318,11 +308,11 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
         // Normally every copy has been consumed. After a timed-out wait, give the stages that may be in
         // flight a bounded chance to land before the block leaves.
         if (!ok)
-            for (uint32_t s = 0; s < p.stages; s++) {
+            for (uint32_t s = 0; s < XV_STAGES; s++) {
                 xv_wait(full(stage), phase ^ 1);
-                if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                if (++stage == XV_STAGES) { stage = 0; phase ^= 1; }
             }
-    } else if (warp < XV_WARPS) {  // ------------------------------------------------------ consumers
+    } else {  // ------------------------------------------------------------------------------- consumers
         const uint32_t g = lane >> 2, t = lane & 3;
         // x in shared memory: [token][step][unit][lane of the quad], tokens 64 bytes apart modulo 128, so
         // that the eight lanes reading at once (two tokens, four quad lanes) reach all 32 banks. Lanes
@@ -338,7 +328,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
 #pragma unroll
         for (int pr = 0; pr < PAIRS; pr++) xs_at[pr] = s_scale + min(2u * pr + (t >> 1), p.m - 1) * p.xsteps;
         const T *x = static_cast<const T *>(p.x);
-        uint32_t stage = 0, phase = 0, turn = 1;
+        uint32_t stage = 0, phase = 0;
         bool ok = true, staged = false;
         uint32_t xphase = 0;
         auto meet = [&]() {
@@ -354,7 +344,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                 if (!staged || p.chunk < p.segs) {
                     // (a bounded meeting: a warp that gave up a wait has left)
                     if (staged && !(ok = meet())) break;
-                    const uint32_t first = c0 * XV_STEPS * 4 * kUnits;
+                    const uint32_t first = c0 * (p.seg / 64) * 4 * kUnits;
                     // Units of x, token after token, four of a thread's loads in flight; whole warps, since a
                     // step's units (16, of E4M3 codes 8) lie in neighbouring lanes and share a power of two.
                     const uint32_t all = p.m * xunits;
@@ -394,24 +384,23 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                 for (uint32_t group = 0; ok && group < w.groups; group++) {
                     float acc[PAIRS][2] = {};
                     for (uint32_t seg = c0; seg < c1; seg++) {
-                        turn ^= 1;
-                        if (turn != warp / XV_TEAM) {  // the other team's stage
-                            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                        if ((stage & 1) != warp / XV_TEAM) {  // the other team's
+                            if (++stage == XV_STAGES) { stage = 0; phase ^= 1; }
                             continue;
                         }
                         if (!xv_wait(full(stage), phase)) { ok = false; break; }
-                        const uint8_t *at = sm + stage * Xv<FMT>::kStage;
-                        const uint32_t steps = (min(p.row_bytes - seg * XV_SEG, (uint32_t)XV_SEG) + 63) / 64;
-                        const uint32_t words = p.words - seg * Xv<FMT>::kWords, x_base = (seg - c0) * XV_STEPS;
+                        const uint8_t *at = sm + stage * p.stage_bytes;
+                        const uint32_t steps = (min(p.row_bytes - seg * p.seg, p.seg) + 63) / 64;
+                        const uint32_t words = p.words - seg * p.seg_words, x_base = (seg - c0) * (p.seg / 64);
                         uint32_t it = warp % XV_TEAM;
                         for (; it + (kU - 1) * XV_TEAM < steps; it += kU * XV_TEAM)
-                            xv_steps<FMT, TY, PAIRS, kU>(at, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
+                            xv_steps<FMT, TY, PAIRS, kU>(at, pitch, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
                         if constexpr (kU > 1)
                             for (; it < steps; it += XV_TEAM)
-                                xv_steps<FMT, TY, PAIRS, 1>(at, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
+                                xv_steps<FMT, TY, PAIRS, 1>(at, pitch, it, x_base + it, g, t, mine, x_at, xs_at, words, xb, acc);
                         __syncwarp();
                         if (lane == 0) mbar_arrive(empty(stage));
-                        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                        if (++stage == XV_STAGES) { stage = 0; phase ^= 1; }
                     }
                     if (!ok) break;
                     // this warp's part of the group, of its own from chunk to chunk
@@ -450,27 +439,36 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
     const uint32_t sms = (uint32_t)device_sms(), grid = quads < sms ? quads : sms;
     p.quads_each = quads / grid;
     p.quads_more = quads % grid;
-    // Shared memory: the partial sums, a ring of 3 or 4 stages, and as much of x as there is room for (at
-    // least a segment: 8 tokens x 2048 E2M1 bytes are 64 KiB).
+    // Shared memory: the partial sums, the ring, and as much of x as there is room for. A stage is 2048 bytes
+    // a row; where all of x does not fit beside four of them, 1536 or 1024 (4 rows of x, 4096 x 14336 MXFP4:
+    // 1536 15.9 us, six stages of 1024 18.7), and beyond that x is walked in chunks (at least a stage's: 8
+    // tokens x 1024 E2M1 bytes are 32 KiB).
     const uint32_t groups = (p.quads_each + (p.quads_more ? 1 : 0) + 3) / 4;
     const size_t sums = (size_t)(groups < (uint32_t)kXvBatch<PAIRS> ? groups : kXvBatch<PAIRS>) * XV_WARPS * 2 * PAIRS * 16 * sizeof(float);
     const size_t step_x = (size_t)p.m * ((FMT == LYTH_MX_FP8 ? 8 : 16) * 16 + (TY == LYTH_NARROW_BF16 ? 4 : 0));
     const uint32_t steps = (p.row_bytes + 63) / 64;
     const size_t room = 226 * 1024 - sums - p.m * 64;
-    p.stages = 4;
-    if (4 * (size_t)Xv<FMT>::kStage + steps * step_x > room) p.stages = 3;
-    const size_t x_room = room - p.stages * (size_t)Xv<FMT>::kStage;
-    p.chunk = steps * step_x <= x_room ? p.segs : (uint32_t)(x_room / (XV_STEPS * step_x));
-    p.xsteps = p.chunk == p.segs ? steps : p.chunk * XV_STEPS;
-    const size_t smem = p.stages * (size_t)Xv<FMT>::kStage + p.xsteps * step_x + p.m * 64 + sums;
-    static size_t set[64] = {0};
+    auto ring = [&](uint32_t seg) {
+        p.seg = seg;
+        p.segs = (p.row_bytes + seg - 1) / seg;
+        p.seg_words = seg / 64 * 2 / (FMT == LYTH_MX_FP8 ? 4 : FMT == LYTH_MX_FP4 ? 2 : 1);
+        p.stage_bytes = 16 * (seg + 64) + p.seg_words * 64;
+        return (size_t)XV_STAGES * p.stage_bytes;
+    };
+    size_t held = ring(2048);
+    if (held + steps * step_x > room) held = ring(1536);
+    if (held + steps * step_x > room) held = ring(1024);
+    p.chunk = held + steps * step_x <= room ? p.segs : (uint32_t)((room - held) / (p.seg / 64 * step_x));
+    p.xsteps = p.chunk == p.segs ? steps : p.chunk * (p.seg / 64);
+    const size_t smem = held + p.xsteps * step_x + p.m * 64 + sums;
+    static bool set[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);
-    if (dev < 0 || dev >= 64 || set[dev] == 0) {
+    if (dev < 0 || dev >= 64 || !set[dev]) {
         e = cudaFuncSetAttribute(mx_gemv_kernel<FMT, TY, PAIRS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
         if (e != cudaSuccess) return status_of(e);
-        if (dev >= 0 && dev < 64) set[dev] = 1;
+        if (dev >= 0 && dev < 64) set[dev] = true;
     }
     mx_gemv_kernel<FMT, TY, PAIRS><<<grid, XV_THREADS, smem, s>>>(p);
     return last_launch_status();
@@ -519,7 +517,6 @@ extern "C" int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32
     p.cols = cols;
     p.row_bytes = (uint32_t)mx_code_bytes(fmt, k);
     p.words = (uint32_t)(k / (4 * mx_block(fmt)));
-    p.segs = (p.row_bytes + XV_SEG - 1) / XV_SEG;
     p.alpha = alpha;
     p.vec = aligned16(x) && ldx * 2 % 16 == 0;
     const bool bf = ty == LYTH_NARROW_BF16;
