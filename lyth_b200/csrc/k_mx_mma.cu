@@ -269,18 +269,24 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
         const uint32_t half = (uint32_t)(warp - 2) >> 2;  // of the steps, then of the columns
         uint32_t stage = half, phase = 0, set = half, old = half, old_phase = 0;
         for (uint32_t kb = k0 + half; kb < k1; kb += 2) {
+            if (!xm_wait(full(stage), phase)) { ok = false; break; }
+            uint4 sa[T], sb[T];  // read while the set may still be in use
+#pragma unroll
+            for (int t = 0; t < T; t++) {
+                sa[t] = *reinterpret_cast<const uint4 *>(sSA + (stage * T + t) * 512 + lane * 16);
+                sb[t] = *reinterpret_cast<const uint4 *>(sSB + (stage * T + t) * 512 + lane * 16);
+            }
             // the set is free once the MMAs of the step X1_SETS back, whose commit frees its stage, are done
             if (kb - k0 >= X1_SETS) {
                 if (!xm_wait(empty(old), old_phase)) { ok = false; break; }
                 if ((old += 2) >= S) { old -= S; old_phase ^= 1; }
             }
-            if (!xm_wait(full(stage), phase)) { ok = false; break; }
             xm_fence_after();
             const uint32_t at = tmem_base + ((quad * 32) << 16) + XM_BN + set * 8 * T;
 #pragma unroll
             for (int t = 0; t < T; t++) {
-                x1_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(sSA + (stage * T + t) * 512 + lane * 16));
-                x1_st4(at + 4 * T + 4 * t, *reinterpret_cast<const uint4 *>(sSB + (stage * T + t) * 512 + lane * 16));
+                x1_st4(at + 4 * t, sa[t]);
+                x1_st4(at + 4 * T + 4 * t, sb[t]);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             xm_fence_before();
@@ -568,6 +574,16 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
         bool ok = true;
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
             for (uint32_t kb = 0; kb < steps; kb++) {
+                if (!xm_wait(sfull(stage), phase)) { ok = false; break; }
+                // a tile is 16 bytes a lane: its words of four columns; read while the set may still be in use
+                const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * NB * T * 512 + lane * 16;
+                uint4 sa[T], sb[T][NB];
+#pragma unroll
+                for (int t = 0; t < T; t++) {
+                    sa[t] = *reinterpret_cast<const uint4 *>(a + t * 512);
+#pragma unroll
+                    for (int h = 0; h < NB; h++) sb[t][h] = *reinterpret_cast<const uint4 *>(b + (h * T + t) * 512);
+                }
                 // the set is free once the MMAs of the step kSets back, whose commit frees its stage, are done
                 if (step >= (uint32_t)kSets) {
                     if (!xm_wait(empty(old), old_phase)) { ok = false; break; }
@@ -575,17 +591,13 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                 } else {
                     step++;
                 }
-                if (!xm_wait(sfull(stage), phase)) { ok = false; break; }
                 xm_fence_after();
                 const uint32_t at = tmem_base + ((quad * 32) << 16) + X2_SF_COL + set * L::kSetCols;
-                // a tile is 16 bytes a lane: its words of four columns
-                const uint8_t *a = sSA + stage * T * 512 + lane * 16, *b = sSB + stage * NB * T * 512 + lane * 16;
 #pragma unroll
                 for (int t = 0; t < T; t++) {
-                    x1_st4(at + 4 * t, *reinterpret_cast<const uint4 *>(a + t * 512));
+                    x1_st4(at + 4 * t, sa[t]);
 #pragma unroll
-                    for (int h = 0; h < NB; h++)
-                        x1_st4(at + 4 * T + 4 * NB * t + 4 * h, *reinterpret_cast<const uint4 *>(b + (h * T + t) * 512));
+                    for (int h = 0; h < NB; h++) x1_st4(at + 4 * T + 4 * NB * t + 4 * h, sb[t][h]);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 xm_fence_before();
