@@ -301,7 +301,7 @@ extern "C" int lyth_b200_quantize_mx(int fmt, int ty, uint64_t rows, uint32_t co
     if (ldx < cols || !mx_tensor_scale(fmt, tensor_scale, inv6g)) return LYTH_E_INVALID;
     if (rows == 0) return LYTH_OK;
     if (!x || !codes || !scales) return LYTH_E_INVALID;
-    if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
+    if (!aligned16(codes) || !aligned16(scales) || !mx_elem_aligned(x, ty)) return LYTH_E_UNSUPPORTED;
     const bool vec = cols % 16 == 0 && aligned32(x) && ldx * mx_ty_bytes(ty) % 32 == 0;
     unsigned grid;
     const MxFlat f = mx_flat(fmt, rows, cols, ldx, vec ? 2 : 1, grid);
@@ -322,7 +322,7 @@ extern "C" int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t 
     if (ldo < cols || !mx_tensor_scale(fmt, tensor_scale, inv6g)) return LYTH_E_INVALID;
     if (rows == 0) return LYTH_OK;
     if (!out || !codes || !scales) return LYTH_E_INVALID;
-    if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
+    if (!aligned16(codes) || !aligned16(scales) || !mx_elem_aligned(out, ty)) return LYTH_E_UNSUPPORTED;
     const bool vec = cols % 16 == 0 && aligned32(out) && ldo * mx_ty_bytes(ty) % 32 == 0;
     unsigned grid;
     const MxFlat f = mx_flat(fmt, rows, cols, ldo, vec ? 2 : 1, grid);
@@ -369,7 +369,9 @@ extern "C" int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t col
         return LYTH_E_INVALID;
     if (rows == 0) return LYTH_OK;
     if (!x || !weight || !codes || !scales) return LYTH_E_INVALID;
-    if (!aligned16(codes) || !aligned16(scales)) return LYTH_E_UNSUPPORTED;
+    if (!aligned16(codes) || !aligned16(scales) || !mx_elem_aligned(x, ty) || !mx_elem_aligned(residual, ty) ||
+        !mx_elem_aligned(residual_out, ty) || !mx_elem_aligned(weight, ty))
+        return LYTH_E_UNSUPPORTED;
     const uint32_t cpr = (uint32_t)(mx_padded(fmt, cols) / kMxChunk);
     const uint64_t size = mx_ty_bytes(ty);
     const bool vec = cols % 16 == 0 && aligned32(x) && ldx * size % 32 == 0 && aligned32(weight) &&

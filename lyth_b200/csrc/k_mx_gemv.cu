@@ -29,7 +29,8 @@
 //
 // Range: bf16 x is brought into f16 by a power of two for each step's columns (128, of E4M3 weights 64
 // neighbouring values of a token; their largest exponent to 2^14) and taken back in f32. Of those values,
-// ones below 2^-32 of the largest lose bits; every other product is exact before the f32 sums.
+// ones below 2^-31 of the largest lose bits (eight bits end at f16's 2^-24); every other product is exact
+// before the f32 sums.
 #include "mbar.cuh"
 #include "mx.cuh"
 
@@ -503,7 +504,8 @@ extern "C" int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32
     if (cols == 0 || cols > (1u << 24) || n > (1u << 31) || ldx < cols || ldy < n) return LYTH_E_INVALID;
     if (m == 0 || n == 0) return LYTH_OK;
     if (!x || !w || !w_scales || !y) return LYTH_E_INVALID;
-    if (!aligned16(w) || !aligned16(w_scales)) return LYTH_E_UNSUPPORTED;
+    if (!aligned16(w) || !aligned16(w_scales) || !mx_elem_aligned(x, ty) || !mx_elem_aligned(y, ty))
+        return LYTH_E_UNSUPPORTED;
     const uint64_t k = mx_padded(fmt, cols);
     XvArgs p;
     p.x = x;

@@ -776,7 +776,8 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     if (cols == 0 || cols > (1u << 30) || m > 0x7FFFFE00u || n > 0x7FFFFE00u || ldc < n) return LYTH_E_INVALID;
     if (m == 0 || n == 0) return LYTH_OK;
     if (!a || !a_scales || !b || !b_scales || !c) return LYTH_E_INVALID;
-    if (!aligned16(a) || !aligned16(a_scales) || !aligned16(b) || !aligned16(b_scales)) return LYTH_E_UNSUPPORTED;
+    if (!aligned16(a) || !aligned16(a_scales) || !aligned16(b) || !aligned16(b_scales) || !mx_elem_aligned(c, ty))
+        return LYTH_E_UNSUPPORTED;
     const uint64_t k = mx_padded(fmt, cols);
     XmArgs p;
     p.sa = a_scales;

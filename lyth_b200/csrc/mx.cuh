@@ -52,6 +52,8 @@ template <> struct MxElem<LYTH_NARROW_BF16> {
 };
 inline bool mx_ty_known(int ty) { return ty == 0 || ty == LYTH_NARROW_F16 || ty == LYTH_NARROW_BF16; }
 inline uint64_t mx_ty_bytes(int ty) { return ty == 0 ? 4 : 2; }
+// Pointers of the unquantised side start on an element (null does).
+inline bool mx_elem_aligned(const void *p, int ty) { return ((uintptr_t)p & (mx_ty_bytes(ty) - 1)) == 0; }
 
 // Two f32 as one register of 16-bit values, a in the low half.
 template <int TY>

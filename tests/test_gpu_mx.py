@@ -469,3 +469,121 @@ def test_no_rows_no_columns_of_the_product(cuda, fmt):
         lb.gemv_mx(fmt, torch.empty(m, 768, dtype=torch.float16, device=cuda), *w, torch.empty(m, 400, dtype=torch.float16, device=cuda))
     lb.matmul_mx(fmt, *w, *lb.mx_empty(fmt, 0, 768, cuda), torch.empty(400, 0, device=cuda))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("cols", [20001, 40001, 40000])  # two chunks a thread; rows read twice, shifted and aligned
+def test_rmsnorm_in_place_of_wide_rows(cuda, fmt, cols):
+    w = torch.ones(cols, dtype=torch.bfloat16, device=cuda)
+    for target in (0, 1):
+        two = [sample(3, cols, torch.bfloat16, 5, cuda), sample(3, cols, torch.bfloat16, 6, cuda)]
+        a, b = empty(fmt, 3, cols, cuda), empty(fmt, 3, cols, cuda)
+        h = torch.empty_like(two[0])
+        lb.rmsnorm_mx(fmt, two[0], w, *a, residual=two[1], residual_out=h)
+        lb.rmsnorm_mx(fmt, two[0], w, *b, residual=two[1], residual_out=two[target])
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        assert torch.equal(two[target].view(torch.int16), h.view(torch.int16))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_one_tensor_in_two_places(cuda, fmt):
+    # x as its own residual; a matrix times itself
+    x = sample(200, 320, torch.bfloat16, 12, cuda)
+    w = torch.ones(320, dtype=torch.bfloat16, device=cuda)
+    a, b = empty(fmt, 200, 320, cuda), empty(fmt, 200, 320, cuda)
+    lb.rmsnorm_mx(fmt, x, w, *a, residual=x)
+    lb.rmsnorm_mx(fmt, x * 2, w, *b)
+    va, vb = torch.empty(200, 320, device=cuda), torch.empty(200, 320, device=cuda)
+    lb.dequantize_mx(fmt, *a, va)
+    lb.dequantize_mx(fmt, *b, vb)
+    assert torch.equal(va, vb)
+    c, d = torch.empty(200, 200, device=cuda), torch.empty(200, 200, device=cuda)
+    lb.matmul_mx(fmt, *a, *a, c)
+    lb.matmul_mx(fmt, *a, *[t.clone() for t in a], d)
+    assert torch.equal(c, d)
+
+
+FIRST = """
+import threading
+import torch
+import lyth_b200 as lb
+
+cuda = torch.device("cuda")
+torch.manual_seed(0)
+x = torch.randn(8, 512, device=cuda).bfloat16()
+xw = torch.randn(20000, 512, device=cuda)
+torch.cuda.synchronize()
+
+
+def buffers():
+    return {"w": lb.mx_empty(1, 20000, 512, cuda), "q": lb.mx_empty(1, 8, 512, cuda), "n": lb.mx_empty(1, 8, 512, cuda),
+            "one": torch.ones(512, dtype=torch.bfloat16, device=cuda), "c": torch.empty(8, 20000, device=cuda),
+            "l": torch.empty(20000, 20000, dtype=torch.bfloat16, device=cuda), "y": torch.empty(8, 20000, dtype=torch.bfloat16, device=cuda),
+            "d": torch.empty(8, 512, device=cuda)}
+
+
+def calls(b):
+    lb.quantize_mx(1, xw, *b["w"])
+    lb.quantize_mx(1, x, *b["q"])
+    lb.dequantize_mx(1, *b["q"], b["d"])
+    lb.rmsnorm_mx(1, x, b["one"], *b["n"])
+    lb.matmul_mx(1, *b["n"], *b["w"], b["c"])
+    lb.matmul_mx(1, *b["w"], *b["w"], b["l"])
+    lb.gemv_mx(1, x, *b["w"], b["y"])
+
+
+def same(a, b):
+    return all(torch.equal(a[k], b[k]) for k in ("c", "l", "y", "d"))
+
+
+MODE
+print("OK")
+"""
+CAPTURED_FIRST = """
+b, want = buffers(), buffers()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls(b)
+g.replay()
+calls(want)
+torch.cuda.synchronize()
+assert same(b, want)
+"""
+THREADS_FIRST = """
+sets, failed = [buffers() for _ in range(4)], []
+torch.cuda.synchronize()
+
+
+def work(b):
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                calls(b)
+            torch.cuda.current_stream().synchronize()
+    except BaseException as e:
+        failed.append(e)
+
+
+threads = [threading.Thread(target=work, args=(b,)) for b in sets]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+assert not failed, failed
+want = buffers()
+calls(want)
+torch.cuda.synchronize()
+assert all(same(b, want) for b in sets)
+"""
+
+
+@pytest.mark.parametrize("mode", [CAPTURED_FIRST, THREADS_FIRST], ids=["captured", "threads"])
+def test_first_calls_of_a_process(cuda, mode):
+    # a process whose first calls are captured, or come from four threads at once
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST.replace("MODE", mode)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("OK"), r.stdout + r.stderr

@@ -79,6 +79,15 @@ def test_unaligned_codes_or_scales(call, names):
         assert call(**{name: ODD}) == lb.E_UNSUPPORTED, name
 
 
+@pytest.mark.parametrize("call,names", [(quantize, ["x"]), (dequantize, ["out"]), (rmsnorm, ["x", "r", "o", "w"]),
+                                        (matmul, ["c"]), (gemv, ["x", "y"])])
+def test_pointers_inside_an_element(call, names):
+    for name in names:
+        assert call(**{name: P + 1}) == lb.E_UNSUPPORTED, name
+        if call is not gemv:
+            assert call(ty=F32, **{name: P + 2}) == lb.E_UNSUPPORTED, name
+
+
 @pytest.mark.parametrize("call,names", [(quantize, ["ldx"]), (dequantize, ["ldo"]), (rmsnorm, ["ldx", "ldr", "ldo"]),
                                         (gemv, ["ldx"])])
 def test_stride_below_the_width(call, names):
