@@ -105,43 +105,134 @@ struct XmArgs {
     bool vec;                // rows of C start on 32 bytes
 };
 
-// A warp's 32 x 32 accumulators (a row a lane) to C, rows row0 .. row0 + 31, columns col .. col + 31.
-// Rows that start on 32 bytes are stored by their lanes in 256-bit pieces, whole sectors; others go
-// through `turn`, the warp's 32 x 17 floats of shared memory, sixteen columns at a time, so that sixteen
-// lanes store a row's neighbouring elements (1001 x 1111 f32, stored by lanes of different rows: 25 us of
-// a product that now takes 10).
-constexpr int XM_TURN = 32 * 17;
+// A lane's row of C, stored 32 columns at a time from left to right. Rows that start on 32 bytes are
+// stored in 256-bit pieces, whole sectors. Others too: a lane shifts its row to the aligned pieces, the
+// end of one chunk completing the next one's first piece; what is left of the first and of the last
+// piece goes out in the few powers of two that make it up. 1500 x 5000 x 1000 MXFP4 to bf16, rows 16
+// bytes off: 14.0 us, first and last bytes by elements 18.2, all through shared memory, so that sixteen
+// lanes stored a row's neighbouring elements, 28.9; rows that start on 32 bytes 10.
+struct XmRow {
+    uint32_t held[8];  // the last chunk of 32 bytes, whose last `delta` bytes are not stored yet
+    bool any = false;
+};
+// a where `on`, else b: in registers (the compiler makes an array in local memory of a chain of choices).
+LYTH_D uint32_t xm_select(uint32_t on, uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tselp.b32 %0, %1, %2, p;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(on));
+    return r;
+}
+// The aligned piece that ends `delta` bytes short of chunk w's end and starts with chunk h's last ones.
+LYTH_D void xm_piece(const uint32_t (&h)[8], const uint32_t (&w)[8], uint32_t delta, uint32_t (&out)[8]) {
+    uint32_t v[12];
+#pragma unroll
+    for (int i = 0; i < 12; i++) {
+        const uint32_t lo = i < 8 ? h[i] : w[i - 8], hi = i < 4 ? h[i + 4] : w[i - 4];
+        v[i] = (32 - delta) & 16 ? hi : lo;
+    }
+    mx_shift<8>(v, (32 - delta) & 15);
+#pragma unroll
+    for (int i = 0; i < 8; i++) out[i] = delta ? v[i] : w[i];
+}
+// The word of a piece that holds byte b.
+LYTH_D uint32_t xm_word(const uint32_t (&w)[8], uint32_t b) {
+    const uint32_t a0 = xm_select(b & 4, w[1], w[0]), a1 = xm_select(b & 4, w[3], w[2]);
+    const uint32_t a2 = xm_select(b & 4, w[5], w[4]), a3 = xm_select(b & 4, w[7], w[6]);
+    return xm_select(b & 16, xm_select(b & 8, a3, a2), xm_select(b & 8, a1, a0));
+}
+// Bytes from .. 31 of the piece at `at`.
+LYTH_D void xm_store_end(char *at, const uint32_t (&w)[8], uint32_t from) {
+    const uint32_t n = 32 - from;
+    if (n & 2) {
+        *reinterpret_cast<uint16_t *>(at + from) = (uint16_t)(xm_word(w, from) >> 16);
+    }
+    if (n & 4) {
+        const uint32_t a = (from + 3) & ~3u;
+        *reinterpret_cast<uint32_t *>(at + a) = xm_word(w, a);
+    }
+    if (n & 8) {
+        const bool up = n >= 16;  // words 2 and 3, else 6 and 7
+        *reinterpret_cast<uint2 *>(at + (up ? 8 : 24)) = up ? make_uint2(w[2], w[3]) : make_uint2(w[6], w[7]);
+    }
+    if (n & 16) *reinterpret_cast<uint4 *>(at + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    if (n & 32) mx_st32(at, w);
+}
+// Bytes 0 .. n - 1 of the piece at `at`, n below 32.
+LYTH_D void xm_store_start(char *at, const uint32_t (&w)[8], uint32_t n) {
+    if (n & 16) *reinterpret_cast<uint4 *>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (n & 8) {
+        const bool up = n & 16;
+        *reinterpret_cast<uint2 *>(at + (up ? 16 : 0)) = up ? make_uint2(w[4], w[5]) : make_uint2(w[0], w[1]);
+    }
+    if (n & 4) {
+        const uint32_t a = n & ~7u;
+        *reinterpret_cast<uint32_t *>(at + a) = xm_word(w, a);
+    }
+    if (n & 2) {
+        const uint32_t a = n & ~3u;
+        *reinterpret_cast<uint16_t *>(at + a) = (uint16_t)xm_word(w, a);
+    }
+}
+// Columns col .. col + 31 of a warp's rows row0 .. (a row a lane), `last` of those that this warp stores.
 template <int TY>
-LYTH_D void xm_store32(typename MxElem<TY>::type *C, uint64_t row0, uint64_t col, const XmArgs &p, float *turn,
+LYTH_D void xm_store32(typename MxElem<TY>::type *C, uint64_t row0, uint64_t col, const XmArgs &p, XmRow &h, bool last,
                        const uint32_t (&r)[32]) {
-    if (col >= p.n) return;
-    const uint32_t lane = threadIdx.x & 31, left = p.n - col < 32 ? (uint32_t)(p.n - col) : 32u;
-    const uint32_t rows = p.m - row0 < 32 ? (uint32_t)(p.m - row0) : 32u;
+    constexpr uint32_t E = TY == 0 ? 4 : 2, kCols = 32 / E;
+    const uint32_t lane = threadIdx.x & 31;
+    if (col >= p.n || row0 + lane >= p.m) return;
+    const uint32_t left = p.n - col < 32 ? (uint32_t)(p.n - col) : 32u;
+    char *to = reinterpret_cast<char *>(C + (row0 + lane) * p.ldc + col);
+    const uint32_t delta = (uint32_t)(reinterpret_cast<uintptr_t>(to) & 31u);
+    uint32_t out[8];
 #pragma unroll
-    for (int v = 0; v < 2; v++) {
-        float f[16];
+    for (uint32_t q = 0; q < 32 / kCols; q++) {
+        if (q * kCols >= left) break;
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) f[i] = __fmul_rn(p.alpha, __uint_as_float(r[16 * v + i]));
-        if (p.vec && 16u * v + 16 <= left) {
-            if (lane < rows) {
-                uint32_t w[kMxWords<TY>];
-                mx_narrow<TY>(f, w);
-                uint32_t *to = reinterpret_cast<uint32_t *>(C + (row0 + lane) * p.ldc + col + 16 * v);
-#pragma unroll
-                for (int i = 0; i < kMxWords<TY>; i += 8) mx_st32(to + i, w + i);
-            }
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t j = q * kCols + i * (4 / E);
+            if constexpr (TY == 0) w[i] = __float_as_uint(__fmul_rn(p.alpha, __uint_as_float(r[j])));
+            else w[i] = mx_pack2<TY>(__fmul_rn(p.alpha, __uint_as_float(r[j])), __fmul_rn(p.alpha, __uint_as_float(r[j + 1])));
+        }
+        const uint32_t bytes = min(left - q * kCols, kCols) * E;
+        if (p.vec && bytes == 32) {
+            mx_st32(to, w);
         } else {
-            __syncwarp();
+            xm_piece(h.held, w, delta, out);
+            if (bytes == 32) {
+                if (h.any) mx_st32(to - delta, out);
+                else xm_store_end(to - delta, out, delta);
 #pragma unroll
-            for (int i = 0; i < 16; i++) turn[lane * 17 + i] = f[i];
-            __syncwarp();
-            const uint32_t c = lane & 15;
-            typename MxElem<TY>::type *to = C + row0 * p.ldc + col + 16 * v + c;
-            if (16u * v + c < left) {
-#pragma unroll 4
-                for (uint32_t i = lane >> 4; i < rows; i += 2) to[(uint64_t)i * p.ldc] = MxElem<TY>::round(turn[i * 17 + c]);
+                for (int i = 0; i < 8; i++) h.held[i] = w[i];
+                h.any = true;
+            } else {  // the row's end
+                uint32_t n = delta + bytes;
+                char *at = to - delta;
+                if (h.any || delta == 0) {
+                    if (n >= 32) {
+                        mx_st32(at, out);
+                        xm_piece(w, w, delta, out);
+                        at += 32;
+                        n -= 32;
+                    }
+                    xm_store_start(at, out, n);
+                } else {  // and its start
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += E) {
+                        if (i < bytes) {
+                            if constexpr (E == 4) *reinterpret_cast<uint32_t *>(to + i) = w[i / 4];
+                            else *reinterpret_cast<uint16_t *>(to + i) = (uint16_t)(w[i / 4] >> (8 * (i & 2)));
+                        }
+                    }
+                }
+                h.any = false;
             }
         }
+        to += 32;
+    }
+    if (h.any && (last || col + 32 >= p.n)) {
+        xm_piece(h.held, h.held, delta, out);
+        xm_store_start(to - delta, out, delta);
+        h.any = false;
     }
 }
 
@@ -302,13 +393,14 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
         const uint32_t r = quad * 32 + lane;
         float *mine = reinterpret_cast<float *>(smem) + r * X1_PITCH;
         if (ok && tm * (uint64_t)XM_BM + quad * 32 < p.m) {
+            XmRow h;
 #pragma unroll 1
             for (uint32_t c = 2 * half; c < 2 * half + 2; c++) {
                 uint32_t v[32];
                 xm_ld32(tmem_base + ((quad * 32) << 16) + c * 32, v);
                 if (ks == 1) {
-                    xm_store32<TY>(C, (uint64_t)tm * XM_BM + quad * 32, (uint64_t)tn * XM_BN + c * 32, p,
-                                   reinterpret_cast<float *>(smem) + (warp - 2) * XM_TURN, v);
+                    xm_store32<TY>(C, (uint64_t)tm * XM_BM + quad * 32, (uint64_t)tn * XM_BN + c * 32, p, h, c & 1, v);
+                    __syncwarp();
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; i++)
@@ -402,9 +494,9 @@ struct X2 {
     static constexpr int kStageBytes = XM_OP_BYTES + NT * X2_B_BYTES + kSfBytes;
     static constexpr int kSetCols = 4 * kTiles * (1 + kBTiles);      // a step's scales in tensor memory
     static constexpr int kSets = 128 / kSetCols < 4 ? 128 / kSetCols : 4;
-    static constexpr int kTurnBytes = 4 * XM_TURN * 4;               // the epilogue's, at 256 bytes past the ring
-    static constexpr int kStages = (227 * 1024 - 1280 - kTurnBytes) / kStageBytes;
-    static constexpr size_t kSmem = 1280 + (size_t)kStages * kStageBytes + kTurnBytes;
+    static constexpr int kStages = (227 * 1024 - 1280) / kStageBytes;
+    static constexpr size_t kSmem = 1280 + (size_t)kStages * kStageBytes;  // 256 bytes of barriers past the ring
+    static_assert((3 * kStages + 4 + 4 + 1) * 8 <= 256, "barriers and the tensor-memory address");
 };
 
 LYTH_D void x2_tma2(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
@@ -610,7 +702,6 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     } else {
         const uint32_t quad = (uint32_t)(warp & 3);  // the TMEM lane quadrant this warp may read
         const uint32_t lead_tempty[2] = {mapa_shared(tempty(0), 0), mapa_shared(tempty(1), 0)};
-        float *turn = reinterpret_cast<float *>(bars + 32) + quad * XM_TURN;
         uint32_t local = 0;
         bool ok = true;
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
@@ -620,11 +711,13 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                 const uint32_t ab = NT == 1 ? local & 1 : h, aphase = NT == 1 ? (local >> 1) & 1 : local & 1;
                 if (!xm_wait(tfull(ab), aphase)) { ok = false; break; }
                 xm_fence_after();
+                XmRow held;
 #pragma unroll 1
                 for (int c = 0; c < X2_BN / 32; c++) {
                     uint32_t r[32];
                     xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
-                    if (row0 < p.m) xm_store32<TY>(C, row0, n0 + h * X2_BN + c * 32, p, turn, r);
+                    xm_store32<TY>(C, row0, n0 + h * X2_BN + c * 32, p, held, c + 1 == X2_BN / 32, r);
+                    __syncwarp();
                 }
                 xm_fence_before();
                 __syncwarp();

@@ -587,3 +587,23 @@ def test_first_calls_of_a_process(cuda, mode):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST.replace("MODE", mode)], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("OK"), r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m", [40, 19000])  # single SMs and CTA pairs
+def test_matmul_rows_of_any_alignment(cuda, ty, m):
+    # the same bits as into rows that start on 32 bytes, and nothing beside them
+    fmt, k = lb.MX_FP8, 128
+    gen = torch.Generator().manual_seed(m)
+    a, b = empty(fmt, m, k, cuda), empty(fmt, 400, k, cuda)
+    lb.quantize_mx(fmt, torch.randn(m, k, generator=gen).to(cuda), *a)
+    lb.quantize_mx(fmt, torch.randn(400, k, generator=gen).to(cuda), *b)
+    want = torch.empty(m, 400, dtype=ty, device=cuda)
+    lb.matmul_mx(fmt, *a, *b, want)
+    for i, n in enumerate([1, 2, 7, 15, 16, 17, 31, 33, 63, 64, 100, 129, 190, 193, 200, 383, 385, 399]):
+        part = b[0][:n].contiguous(), b[1][:(n + 127) // 128 * 512 * (k // 128)].contiguous()
+        for off, pad in ((i % 17, 1), ((5 * i + 3) % 16, (7 * i) % 16), (8, 16 - n % 16)):
+            full = torch.full((m, off + n + pad), 3.0, dtype=ty, device=cuda)
+            lb.matmul_mx(fmt, *a, *part, full[:, off:off + n])
+            assert torch.equal(full[:, off:off + n], want[:, :n]), (n, off, pad)
+            assert bool((full[:, :off] == 3).all()) and bool((full[:, off + n:] == 3).all()), (n, off, pad)
