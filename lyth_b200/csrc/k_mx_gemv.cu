@@ -8,9 +8,9 @@
 // (token, lane of the quad), and x stands only where the column's lane is the lane that holds those k,
 // zero elsewhere. A column's sum then is one lane's part, of one scale block, and is multiplied by
 // that block's scale in f32 afterwards: four multiply-adds for the 64 codes a lane holds. Tensor-core
-// work is four times what the product needs and is idle capacity here.
+// work is four times what the product needs and is idle capacity for one or two tokens.
 //
-// What bounds the arithmetic is the conversion of codes (two codes an instruction, at half the issue
+// What bounds the arithmetic of those is the conversion of codes (two codes an instruction, at half the issue
 // rate), so everything around it is kept off the warps that convert: one block per SM, in roles:
 //   producers (4 warps)  bring a stage -- 16 rows of W, up to 2048 bytes of each, and their scale words --
 //                        into a ring of shared-memory stages, four rows a warp: a bulk copy per row (one
@@ -25,7 +25,10 @@
 // Every mbarrier wait is bounded (mbar.cuh); one that runs out sets the device error flag and the
 // block winds down. Loading and converting in the same warps, with four steps of loads in flight in
 // registers, took 13.2 us for one token through 14336 x 4096 NVFP4 weights: 9.5 us without the loads,
-// 10.6 us without the arithmetic.
+// 10.6 us without the arithmetic. Now: one token through 14336 x 4096 NVFP4 11.1 us (33 MB, 3.0 TB/s),
+// MXFP8 14.2 (4.3 TB/s), four tokens 16, eight 25.7, where the tensor-core steps bound it. Eight tokens as
+// the columns of one step, W's codes times their scales in f16, took 18.6, but a token's sum then had other
+// roundings than alone; taken for every count it cost one token 12.7.
 //
 // Range: bf16 x is brought into f16 by a power of two for each step's columns (128, of E4M3 weights 64
 // neighbouring values of a token; their largest exponent to 2^14) and taken back in f32. Of those values,

@@ -241,7 +241,8 @@ LYTH_D void xm_store32(typename MxElem<TY>::type *C, uint64_t row0, uint64_t col
 // takes a tile, each a contiguous share of k, so that few tiles still fill the machine; their
 // accumulators meet in shared memory and every CTA adds up a share of the columns over the cluster, in
 // rank order. One token batch of 32 through 14336 x 4096 is 112 tiles; through 4096 x 14336, 32 tiles
-// of four shares.
+// of four shares. NVFP4, 34 MB: 10 and 11 us, 3.3 TB/s; start, first copies and the epilogue are about
+// four of them, and a quarter of the SMs have no tile.
 //   warp 0     producer: boxes of A (only the rows that exist), B and both operands' scales.
 //   warp 1     issues the MMAs.
 //   warps 2-9  scales from shared to tensor memory as below, four warps the even steps and four the odd
@@ -468,6 +469,8 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
 // accumulators (2 x 192) beside two sets of scales. NT = 1: the accumulators take turns, and the
 // epilogue of a tile runs beside the next. NT = 2: a tile of 256 x 384 uses both, a third less traffic
 // for the work, with the epilogue partly exposed; chosen where it leaves fewer rounds (launch rule).
+// Measured: 4096 x 14336 x 4096 NVFP4 105 us (4.6 PFLOP/s), MXFP4 100; 4096^3 NVFP4 38 us (3.7), MXFP4
+// 34 to 36, MXFP8 57 (2.4 PFLOP/s).
 //
 //   both CTAs, warp 0    producer: its halves of A and B as boxes that complete on the leader's `full`
 //                        barrier; its 128 rows' A scales and the B scales of all 192 columns (the pair's
@@ -886,8 +889,9 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
     if (tiles > (uint64_t)device_sms()) {
         // Rounds of all pairs over the tiles: of 192 columns, or of 384, whose round is twice the work in 0.85
-        // (NVFP4; 0.9 of the others) of twice the time. 4096 x 14336 x 4096: 17 rounds against 9, 123 and
-        // 108 us; 4096^3 MXFP4: 5 against 3, 35 and 38 us.
+        // (NVFP4; 0.9 of the others) of twice the time. 4096 x 14336 x 4096 NVFP4: 17 rounds against 9,
+        // 116 and 106 us; 8192 x 4096 x 14336 MXFP8: 10 against 5, 435 and 358; 4096^3 MXFP4: 5 against 3,
+        // 35.6 and 38.5; 2048 x 4096 x 4096 MXFP8: 3 against 2, 34 and 41.
         const uint64_t pairs = (uint64_t)device_sms() / 2, rows = ((uint64_t)m + 255) / 256;
         const uint64_t one = (rows * (((uint64_t)n + X2_BN - 1) / X2_BN) + pairs - 1) / pairs;
         const uint64_t two = (rows * (((uint64_t)n + 2 * X2_BN - 1) / (2 * X2_BN)) + pairs - 1) / pairs;
