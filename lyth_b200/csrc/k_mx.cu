@@ -48,8 +48,11 @@ template <int FMT, int TY, bool VEC, int U>
 __global__ void __launch_bounds__(kMxThreads)
     mx_quantize_kernel(const typename MxElem<TY>::type *__restrict__ x, MxFlat f, float inv6g, float g,
                        uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    grid_next();
     const uint32_t words = f.cpr * 16 / Mx<FMT>::kWord;
     const uint64_t row_bytes = (uint64_t)f.cpr * 2 * Mx<FMT>::kBits;
+    grid_wait();
+    x = after_wait(x);
     const void *hi = x + (f.rows - 1) * f.ld + f.cols;
     MxWalk w((uint64_t)blockIdx.x * (kMxThreads * U) + threadIdx.x, f.cpr, f.narrow);
     uint64_t row[U];
@@ -82,7 +85,11 @@ __global__ void __launch_bounds__(kMxThreads)
     const uint32_t words = f.cpr * 16 / Mx<FMT>::kWord;
     constexpr int kLanes = Mx<FMT>::kBlock / 16, kW = Mx<FMT>::kBits / 2;  // lanes of a block, words of a chunk
     const uint64_t flat = (uint64_t)blockIdx.x * (kMxThreads * U) + threadIdx.x;
+    grid_next();
     MxWalk w(flat, f.cpr, f.narrow);
+    grid_wait();
+    codes = after_wait(codes);
+    scales = after_wait(scales);
     uint64_t row[U];
     uint32_t c[U], in[U][kW], byte[U];
 #pragma unroll
@@ -150,6 +157,11 @@ __global__ void __launch_bounds__(1024)
                       float inv6g, float g, uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
     constexpr int N = kMxWords<TY>, kHeld = V > 0 ? V : 1;
     __shared__ float part[32];
+    grid_next();
+    grid_wait();
+    x = after_wait(x);
+    residual = after_wait(residual);
+    weight = after_wait(weight);
     const uint32_t tpr = blockDim.x, warps = tpr >> 5;
     const uint32_t words = cpr * 16 / Mx<FMT>::kWord;
     const uint64_t row_bytes = (uint64_t)cpr * 2 * Mx<FMT>::kBits, step = (uint64_t)gridDim.x * blockDim.y;
@@ -311,9 +323,9 @@ extern "C" int lyth_b200_quantize_mx(int fmt, int ty, uint64_t rows, uint32_t co
     if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
                      auto k = vec ? mx_quantize_kernel<FMT, TY, true, 2> : mx_quantize_kernel<FMT, TY, false, 1>;
-                     k<<<grid, kMxThreads, 0, s>>>(static_cast<const MxElem<TY>::type *>(x), f, inv6g, tensor_scale,
-                                                   codes, scales));
-    return last_launch_status();
+                     return mx_launch(k, grid, kMxThreads, 0, s, 1, static_cast<const MxElem<TY>::type *>(x), f,
+                                                inv6g, tensor_scale, codes, scales));
+    return LYTH_E_UNSUPPORTED;
 }
 
 extern "C" int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const uint8_t *codes,
@@ -332,8 +344,9 @@ extern "C" int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t 
     if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
                      auto k = vec ? mx_dequantize_kernel<FMT, TY, true, 2> : mx_dequantize_kernel<FMT, TY, false, 1>;
-                     k<<<grid, kMxThreads, 0, s>>>(codes, scales, f, tensor_scale, static_cast<MxElem<TY>::type *>(out)));
-    return last_launch_status();
+                     return mx_launch(k, grid, kMxThreads, 0, s, 1, codes, scales, f, tensor_scale,
+                                                static_cast<MxElem<TY>::type *>(out)));
+    return LYTH_E_UNSUPPORTED;
 }
 
 template <int FMT, int TY>
@@ -356,8 +369,8 @@ static int rmsnorm_launch(const void *x, const void *residual, void *residual_ou
     auto k = v == 1   ? (vec ? mx_rmsnorm_kernel<FMT, TY, 1, true> : mx_rmsnorm_kernel<FMT, TY, 1, false>)
              : v == 2 ? (vec ? mx_rmsnorm_kernel<FMT, TY, 2, true> : mx_rmsnorm_kernel<FMT, TY, 2, false>)
                       : (vec ? mx_rmsnorm_kernel<FMT, TY, 0, true> : mx_rmsnorm_kernel<FMT, TY, 0, false>);
-    k<<<grid, block, 0, s>>>(xt, rt, ot, wt, rows, cols, ldx, ldr, ldo, cpr, eps, inv6g, g, codes, scales);
-    return last_launch_status();
+    return mx_launch(k, grid, block, 0, s, 1, xt, rt, ot, wt, rows, cols, ldx, ldr, ldo, cpr, eps, inv6g, g, codes,
+                               scales);
 }
 
 extern "C" int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const void *x, uint64_t ldx,

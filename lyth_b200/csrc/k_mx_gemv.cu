@@ -267,6 +267,8 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    grid_next();
+    grid_wait();
 
     if (warp >= XV_WARPS) {  // ------------------------------------------------------------------ producers
         uint32_t stage = 0, phase = 0;
@@ -474,8 +476,7 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
         if (e != cudaSuccess) return status_of(e);
         if (dev >= 0 && dev < 64) set[dev] = true;
     }
-    mx_gemv_kernel<FMT, TY, PAIRS><<<grid, XV_THREADS, smem, s>>>(p);
-    return last_launch_status();
+    return mx_launch(mx_gemv_kernel<FMT, TY, PAIRS>, grid, XV_THREADS, smem, s, 1, p);
 }
 
 template <int FMT, int TY>

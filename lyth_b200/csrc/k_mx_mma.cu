@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
     const uint32_t tiles_m = (uint32_t)((p.m + XM_BM - 1) / XM_BM), tm = tile % tiles_m, tn = tile / tiles_m;
     const uint32_t all = (p.row_bytes + 127) / 128, k0 = all * rank / ks, k1 = all * (rank + 1) / ks;
 
+    grid_next();
     if (threadIdx.x == 32) {
         xm_prefetch(&tmA);
         xm_prefetch(&tmB);
@@ -308,6 +309,7 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
     __syncthreads();
     xm_fence_after();
     const uint32_t tmem_base = warp_uniform(*tmem_slot);
+    grid_wait();
     bool ok = true;
 
     if (warp == 0) {
@@ -553,6 +555,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + NT * X2_BN - 1) / (NT * X2_BN), ntiles = tiles_m * tiles_n;
     const uint32_t steps = (p.row_bytes + 127) / 128;
 
+    grid_next();
     if (threadIdx.x == 32) {
         xm_prefetch(&tmA);
         xm_prefetch(&tmB);
@@ -582,6 +585,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
     cluster_sync_all();
     xm_fence_after();
     const uint32_t tmem_base = warp_uniform(*tmem_slot);
+    grid_wait();
 
     if (warp == 0) {
         uint32_t stage = 0, phase = 0;
@@ -777,21 +781,20 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(X2_THREADS);
-    cfg.dynamicSmemBytes = L::kSmem;
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     int pairs = device_sms() / 2;
     if (dev < 0 || dev >= 64 || fit_of[dev] == 0) {
         e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
         if (e != cudaSuccess) return status_of(e);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.blockDim = dim3(X2_THREADS);
+        cfg.dynamicSmemBytes = L::kSmem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
         cfg.gridDim = dim3(2u * (unsigned)pairs);
         int fit = 0;
         if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY, NT>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
@@ -803,10 +806,8 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     }
     const uint64_t tiles = (p.m + 255) / 256 * ((p.n + NT * X2_BN - 1) / (NT * X2_BN));
     if ((uint64_t)pairs > tiles) pairs = (int)tiles;
-    cfg.gridDim = dim3(2u * (unsigned)pairs);
-    e = cudaLaunchKernelEx(&cfg, mx_mma2_kernel<FMT, TY, NT>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p);
-    if (e != cudaSuccess) return status_of(e);
-    return last_launch_status();
+    return mx_launch(mx_mma2_kernel<FMT, TY, NT>, 2u * (unsigned)pairs, X2_THREADS, L::kSmem, s, 2, ta, tb, tsa, tsb,
+                               static_cast<typename MxElem<TY>::type *>(c), p);
 }
 
 template <int FMT, int TY>
@@ -833,22 +834,8 @@ static int x1_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     const uint32_t steps = (p.row_bytes + 127) / 128;
     uint32_t klog = 0;
     while (klog < 2 && tiles << (klog + 1) <= (uint32_t)device_sms() && steps >> (klog + 1) >= 4) klog++;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1u << klog;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(tiles << klog);
-    cfg.blockDim = dim3(X1_THREADS);
-    cfg.dynamicSmemBytes = Xm<FMT>::kSmem;
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, mx_mma1_kernel<FMT, TY>, ta, tb, tsa, tsb, static_cast<typename MxElem<TY>::type *>(c), p,
-                           klog, a_rows);
-    if (e != cudaSuccess) return status_of(e);
-    return last_launch_status();
+    return mx_launch(mx_mma1_kernel<FMT, TY>, tiles << klog, X1_THREADS, Xm<FMT>::kSmem, s, 1u << klog, ta, tb, tsa,
+                               tsb, static_cast<typename MxElem<TY>::type *>(c), p, klog, a_rows);
 }
 
 int mx_take_device_error() {

@@ -36,6 +36,42 @@ inline uint64_t mx_padded(int fmt, uint64_t cols) {
 }
 inline uint64_t mx_code_bytes(int fmt, uint64_t k) { return fmt == LYTH_MX_FP8 ? k : k / 2; }
 
+// ---- launches that overlap. A kernel here may be placed on the SMs while the one before it in the stream
+// still runs its last blocks: all that touches no tensor (barriers, tensor memory, indexes) comes before
+// grid_wait(), which returns once every earlier grid of the stream is complete and its writes are visible;
+// grid_next() lets the following kernel do the same. Every thread that reads or writes global memory
+// waits, and loads are not hoisted above it: pointers pass through grid_wait, or the loads are volatile.
+LYTH_D void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename T>
+LYTH_D T *after_wait(T *p) {  // p, as a value that exists only once the wait is over
+    asm volatile("" : "+l"(p)::"memory");
+    return p;
+}
+LYTH_D void grid_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Host: a launch with that leave, as clusters of `cluster` blocks; its status.
+template <typename... P, typename... A>
+inline int mx_launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, unsigned cluster,
+                             A... args) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by the next call
+    return status_of(e);
+}
+
 // ---- element types of the unquantised side: 0 f32, LYTH_NARROW_F16, LYTH_NARROW_BF16.
 template <int TY> struct MxElem;
 template <> struct MxElem<0> {

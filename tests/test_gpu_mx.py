@@ -607,3 +607,72 @@ def test_matmul_rows_of_any_alignment(cuda, ty, m):
             lb.matmul_mx(fmt, *a, *part, full[:, off:off + n])
             assert torch.equal(full[:, off:off + n], want[:, :n]), (n, off, pad)
             assert bool((full[:, :off] == 3).all()) and bool((full[:, off + n:] == 3).all()), (n, off, pad)
+
+
+def chain(x, s, between):
+    # every call reads what the one before it has just written, others' kernels and copies between them
+    fmt = lb.MX_FP8
+    for _ in range(3):
+        lb.rmsnorm_mx(fmt, x, s["one"], *s["n"], residual=s["r"], residual_out=s["r"])
+        between()
+        lb.matmul_mx(fmt, *s["n"], *s["w"], s["c"], alpha=0.05)
+        between()
+        lb.quantize_mx(fmt, s["c"], *s["q"])
+        between()
+        lb.matmul_mx(fmt, *s["q"], *s["w"], s["d"], alpha=0.05)
+        between()
+        s["e"].copy_(s["d"])
+        between()
+        lb.gemv_mx(fmt, s["e"][:8], *s["w"], x[:8], alpha=0.05)
+        between()
+        lb.quantize_mx(fmt, x, *s["n"])
+        between()
+        lb.dequantize_mx(fmt, *s["n"], x)
+        between()
+        x.add_(s["e"])
+        between()
+
+
+@pytest.mark.parametrize("rows", [8, 300, 5000])
+def test_a_chain_of_dependent_calls(cuda, rows):
+    k = 512
+    gen = torch.Generator().manual_seed(rows)
+    start, r = torch.randn(rows, k, generator=gen).bfloat16().to(cuda), torch.randn(rows, k, generator=gen).bfloat16().to(cuda)
+    s = {"one": torch.ones(k, dtype=torch.bfloat16, device=cuda), "n": empty(lb.MX_FP8, rows, k, cuda), "q": empty(lb.MX_FP8, rows, k, cuda),
+         "w": empty(lb.MX_FP8, k, k, cuda), "c": torch.empty(rows, k, device=cuda), "d": torch.empty(rows, k, device=cuda),
+         "e": torch.empty(rows, k, dtype=torch.bfloat16, device=cuda), "r": r.clone()}
+    lb.quantize_mx(lb.MX_FP8, torch.randn(k, k, generator=gen).to(cuda), *s["w"])
+    want = start.clone()
+    chain(want, s, torch.cuda.synchronize)
+    want_r = s["r"].clone()
+    for _ in range(20):
+        x = start.clone()
+        s["r"].copy_(r)
+        chain(x, s, lambda: None)
+        assert torch.equal(x, want) and torch.equal(s["r"], want_r)
+    # captured, with a second stream's work joined in the middle
+    x, side = start.clone(), torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    y = torch.empty_like(x)
+    with torch.cuda.graph(g):
+        x.copy_(start)
+        s["r"].copy_(r)
+        chain(x, s, lambda: None)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            lb.quantize_mx(lb.MX_FP8, s["c"], *s["q"])
+            y.copy_(x)
+        lb.quantize_mx(lb.MX_FP8, x, *s["n"])
+        torch.cuda.current_stream().wait_stream(side)
+        lb.dequantize_mx(lb.MX_FP8, *s["q"], s["d"])
+        lb.dequantize_mx(lb.MX_FP8, *s["n"], s["e"])
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, want) and torch.equal(y, want) and torch.equal(s["r"], want_r)
+    for src, (codes, scales), got in ((s["c"], s["q"], s["d"]), (x, s["n"], s["e"])):
+        again, out = empty(lb.MX_FP8, rows, k, cuda), torch.empty_like(got)
+        lb.quantize_mx(lb.MX_FP8, src, *again)
+        torch.cuda.synchronize()
+        lb.dequantize_mx(lb.MX_FP8, *again, out)
+        assert torch.equal(codes, again[0]) and torch.equal(got, out)
