@@ -448,11 +448,15 @@ def _mx_on(t, name, dev):
 
 
 def _mx_rows(t, name, dev, dtype=None):
-    """(pointer, row stride) of a 2-D CUDA tensor whose rows are contiguous; any row stride."""
-    _mx_on(t, name, dev)
+    """(rows, columns, pointer, row stride) of a 2-D CUDA tensor whose rows are contiguous; any row stride."""
+    if t.get_device() != dev:
+        _mx_on(t, name, dev)
     if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    rows, cols = t.shape
+    try:
+        rows, cols = t.shape
+    except ValueError:
+        raise ValueError(f"{name}: expected two dimensions, got {t.dim()}") from None
     ld, inner = t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name}: rows must be contiguous")
@@ -460,13 +464,14 @@ def _mx_rows(t, name, dev, dtype=None):
         ld = cols
     elif ld < cols:
         raise ValueError(f"{name}: rows overlap (stride {ld}, width {cols})")
-    return t.data_ptr(), ld
+    return rows, cols, t.data_ptr(), ld
 
 
 def _mx_operand(fmt, rows, cols, codes, scales, dev, name):
     """Pointers of a quantised rows x cols matrix, its sizes checked against the format's."""
-    _mx_on(codes, name, dev)
-    _mx_on(scales, name + "'s scales", dev)
+    if codes.get_device() != dev or scales.get_device() != dev:
+        _mx_on(codes, name, dev)
+        _mx_on(scales, name + "'s scales", dev)
     if codes.dtype is not _mx_u8 or scales.dtype is not _mx_u8:
         raise TypeError(f"{name}: codes and scales are uint8, got {codes.dtype} and {scales.dtype}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
@@ -483,18 +488,11 @@ def _mx_operand(fmt, rows, cols, codes, scales, dev, name):
     return codes.data_ptr(), scales.data_ptr()
 
 
-def _mx_shape(t, name):
-    if t.dim() != 2:
-        raise ValueError(f"{name}: expected two dimensions, got {t.dim()}")
-    return t.shape
-
-
 def quantize_mx(fmt: int, x, codes, scales, tensor_scale: float = 1.0, stream=None) -> None:
     """codes, scales = x in a block-scaled format; x 2-D float32 / float16 / bfloat16 with contiguous
     rows (any row stride), codes and scales as mx_empty gives them. tensor_scale: NVFP4 only."""
     dev = _mx_device()
-    rows, cols = _mx_shape(x, "x")
-    xp, ldx = _mx_rows(x, "x", dev)
+    rows, cols, xp, ldx = _mx_rows(x, "x", dev)
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
     check(lib.lyth_b200_quantize_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, tensor_scale, cp, sp, _mx_stream(stream, dev)),
           "quantize_mx")
@@ -503,8 +501,7 @@ def quantize_mx(fmt: int, x, codes, scales, tensor_scale: float = 1.0, stream=No
 def dequantize_mx(fmt: int, codes, scales, out, tensor_scale: float = 1.0, stream=None) -> None:
     """out = the values codes and scales stand for, rounded once to out's type."""
     dev = _mx_device()
-    rows, cols = _mx_shape(out, "out")
-    op, ldo = _mx_rows(out, "out", dev)
+    rows, cols, op, ldo = _mx_rows(out, "out", dev)
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
     check(lib.lyth_b200_dequantize_mx(fmt, _mx_ty(out, "out"), rows, cols, cp, sp, tensor_scale, op, ldo,
                                       _mx_stream(stream, dev)), "dequantize_mx")
@@ -515,22 +512,24 @@ def rmsnorm_mx(fmt: int, x, weight, codes, scales, residual=None, residual_out=N
     """h = x + residual (f32); codes, scales = h / sqrt(mean(h^2) + eps) * weight quantised;
     residual_out = h rounded to x's type (it may be x or residual itself)."""
     dev = _mx_device()
-    rows, cols = _mx_shape(x, "x")
-    xp, ldx = _mx_rows(x, "x", dev)
+    rows, cols, xp, ldx = _mx_rows(x, "x", dev)
     rp = op = None
     ldr = ldo = 0
-    for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None and t.shape != (rows, cols):
-            raise ValueError(f"{name}: expected {rows} x {cols}, got {tuple(t.shape)}")
+    dtype = x.dtype
     if residual is not None:
-        rp, ldr = _mx_rows(residual, "residual", dev, x.dtype)
+        r_rows, r_cols, rp, ldr = _mx_rows(residual, "residual", dev, dtype)
+        if r_rows != rows or r_cols != cols:
+            raise ValueError(f"residual: expected {rows} x {cols}, got {r_rows} x {r_cols}")
     if residual_out is not None:
-        op, ldo = _mx_rows(residual_out, "residual_out", dev, x.dtype)
-    _mx_on(weight, "weight", dev)
+        o_rows, o_cols, op, ldo = _mx_rows(residual_out, "residual_out", dev, dtype)
+        if o_rows != rows or o_cols != cols:
+            raise ValueError(f"residual_out: expected {rows} x {cols}, got {o_rows} x {o_cols}")
+    if weight.get_device() != dev:
+        _mx_on(weight, "weight", dev)
     if weight.shape != (cols,) or not weight.is_contiguous():
         raise ValueError(f"weight: expected {cols} values, contiguous, got {tuple(weight.shape)}")
-    if weight.dtype is not x.dtype:
-        raise TypeError(f"weight: expected {x.dtype}, got {weight.dtype}")
+    if weight.dtype is not dtype:
+        raise TypeError(f"weight: expected {dtype}, got {weight.dtype}")
     cp, sp = _mx_operand(fmt, rows, cols, codes, scales, dev, "codes")
     check(lib.lyth_b200_rmsnorm_mx(fmt, _mx_ty(x, "x"), rows, cols, xp, ldx, rp, ldr, op, ldo,
                                    weight.data_ptr(), eps, tensor_scale, cp, sp, _mx_stream(stream, dev)),
@@ -541,9 +540,10 @@ def matmul_mx(fmt: int, a, a_scales, b, b_scales, c, alpha: float = 1.0, stream=
     """c = alpha * a @ b.T on the block-scaled tensor cores: a (m rows) and b (n rows) are codes in one
     format and of one width, c m x n float32 / float16 / bfloat16 with contiguous rows."""
     dev = _mx_device()
-    m, n = _mx_shape(c, "c")
-    cols = _mx_shape(a, "a")[1] << (fmt != MX_FP8)
-    cp, ldc = _mx_rows(c, "c", dev)
+    m, n, cp, ldc = _mx_rows(c, "c", dev)
+    if a.dim() != 2:
+        raise ValueError(f"a: expected two dimensions, got {a.dim()}")
+    cols = a.shape[1] << (fmt != MX_FP8)
     ap, asp = _mx_operand(fmt, m, cols, a, a_scales, dev, "a")
     bp, bsp = _mx_operand(fmt, n, cols, b, b_scales, dev, "b")
     check(lib.lyth_b200_matmul_mx(fmt, _mx_ty(c, "c"), m, n, cols, ap, asp, bp, bsp, alpha, cp, ldc, _mx_stream(stream, dev)),
@@ -554,12 +554,10 @@ def gemv_mx(fmt: int, x, w, w_scales, y, alpha: float = 1.0, stream=None) -> Non
     """y = alpha * x @ w.T for up to GEMV_MX_MAX_M rows of float16 / bfloat16 x (m x cols); w holds
     n x cols in a block-scaled format, y is m x n of x's type."""
     dev = _mx_device()
-    m, cols = _mx_shape(x, "x")
-    m2, n = _mx_shape(y, "y")
+    m, cols, xp, ldx = _mx_rows(x, "x", dev)
+    m2, n, yp, ldy = _mx_rows(y, "y", dev, x.dtype)
     if m2 != m:
         raise ValueError(f"gemv shapes {tuple(x.shape)} -> {tuple(y.shape)}")
-    xp, ldx = _mx_rows(x, "x", dev)
-    yp, ldy = _mx_rows(y, "y", dev, x.dtype)
     wp, wsp = _mx_operand(fmt, n, cols, w, w_scales, dev, "w")
     check(lib.lyth_b200_gemv_mx(fmt, _mx_ty(x, "x"), m, n, cols, xp, ldx, wp, wsp, alpha, yp, ldy, _mx_stream(stream, dev)),
           "gemv_mx")
