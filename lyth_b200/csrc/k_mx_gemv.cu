@@ -25,10 +25,10 @@
 // Every mbarrier wait is bounded (mbar.cuh); one that runs out sets the device error flag and the
 // block winds down. Loading and converting in the same warps, with four steps of loads in flight in
 // registers, took 13.2 us for one token through 14336 x 4096 NVFP4 weights: 9.5 us without the loads,
-// 10.6 us without the arithmetic. Now: one token through 14336 x 4096 NVFP4 11.1 us (33 MB, 3.0 TB/s),
-// MXFP8 14.2 (4.3 TB/s), four tokens 16, eight 25.7, where the tensor-core steps bound it. Eight tokens as
-// the columns of one step, W's codes times their scales in f16, took 18.6, but a token's sum then had other
-// roundings than alone; taken for every count it cost one token 12.7.
+// 10.6 us without the arithmetic. Now: one token through 14336 x 4096 NVFP4 10.6 us (33 MB, 3.1 TB/s),
+// MXFP8 13.5 (4.5 TB/s), four tokens 15, eight 25, where the tensor-core steps bound it. Eight tokens as
+// the columns of one step, W's codes times their scales in f16, took 18.6 (this then 25.7), but a token's sum then had other
+// roundings than alone; taken for every count it cost one token 12.7 instead of 11.1.
 //
 // Range: bf16 x is brought into f16 by a power of two for each step's columns (128, of E4M3 weights 64
 // neighbouring values of a token; their largest exponent to 2^14) and taken back in f32. Of those values,

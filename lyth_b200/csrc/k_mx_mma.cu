@@ -241,8 +241,8 @@ LYTH_D void xm_store32(typename MxElem<TY>::type *C, uint64_t row0, uint64_t col
 // takes a tile, each a contiguous share of k, so that few tiles still fill the machine; their
 // accumulators meet in shared memory and every CTA adds up a share of the columns over the cluster, in
 // rank order. One token batch of 32 through 14336 x 4096 is 112 tiles; through 4096 x 14336, 32 tiles
-// of four shares. NVFP4, 34 MB: 10 and 11 us, 3.3 TB/s; start, first copies and the epilogue are about
-// four of them, and a quarter of the SMs have no tile.
+// of four shares. NVFP4, 34 MB: 9.9 us, MXFP4 10.0, 3.4 TB/s; first copies and the epilogue are about four
+// of them, and a quarter of the SMs have no tile.
 //   warp 0     producer: boxes of A (only the rows that exist), B and both operands' scales.
 //   warp 1     issues the MMAs.
 //   warps 2-9  scales from shared to tensor memory as below, four warps the even steps and four the odd
