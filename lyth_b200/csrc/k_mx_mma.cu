@@ -4,7 +4,7 @@
 // inside the contraction, so nothing is dequantised.
 //
 // Two forms, chosen by the number of 128 x 128 tiles: up to one per SM, single SMs whose clusters share k
-// (mx_mma1_kernel); more, CTA pairs on 256 x 192 tiles (mx_mma2_kernel). Both stage steps of 128 bytes
+// (mx_mma1_kernel); more, CTA pairs on tiles of 256 x 192 to 384 (mx_mma2_kernel). Both stage steps of 128 bytes
 // along k (128 E4M3 or 256 E2M1 codes) of A and B in a shared-memory ring (TMA, 128-byte swizzle, no
 // multicast) with both operands' scale tiles (512 bytes per 128 rows x 4 blocks, already in the order
 // tensor memory wants), move the scales to tensor memory and issue one MMA per 32 bytes of k.
@@ -468,11 +468,12 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
 // its 128 rows of A and 96 of the tile's 192 rows of B, so a 128-byte step moves 28 KiB into an SM for
 // the work that takes the 128 x 128 form 42 KiB: at 4 bits it is this traffic that bounds, 47 bytes a
 // cycle into an SM measured, not the tensor cores. 192 columns leave room in tensor memory for two
-// accumulators (2 x 192) beside two sets of scales. NT = 1: the accumulators take turns, and the
+// accumulators (2 x 192) beside the sets of scales. NT = 1: the accumulators take turns, and the
 // epilogue of a tile runs beside the next. NT = 2: a tile of 256 x 384 uses both, a third less traffic
-// for the work, with the epilogue partly exposed; chosen where it leaves fewer rounds (launch rule).
-// Measured: 4096 x 14336 x 4096 NVFP4 105 us (4.6 PFLOP/s), MXFP4 100; 4096^3 NVFP4 38 us (3.7), MXFP4
-// 34 to 36, MXFP8 57 (2.4 PFLOP/s).
+// for the work, with the epilogue partly exposed. BN = 256: one accumulator of 256 columns, the epilogue
+// exposed. Chosen by the rounds that each leaves (launch rule).
+// Measured: 4096 x 14336 x 4096 NVFP4 105 us (4.6 PFLOP/s), MXFP4 99; 4096^3 NVFP4 34.5 us (4.0), MXFP4
+// 33, MXFP8 57 (2.4 PFLOP/s).
 //
 //   both CTAs, warp 0    producer: its halves of A and B as boxes that complete on the leader's `full`
 //                        barrier; its 128 rows' A scales and the B scales of all 192 columns (the pair's
@@ -484,21 +485,23 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
 //   leader, warp 1       issues the MMAs; one commit frees the stage, and the set of scales in tensor
 //                        memory, in both CTAs.
 //   both CTAs, warps 2-5 epilogue of this CTA's 128 rows.
-// B scale tiles are 128 rows and the tile's 192 start on a multiple of 64: two tiles cover them, and
+// B scale tiles are 128 rows and a tile of 192 starts on a multiple of 64: two scale tiles cover it, and
 // an odd start reads from two tensor-memory columns (64 rows) on.
-constexpr int X2_BN = 192, X2_HALF = X2_BN / 2;
-constexpr int X2_B_BYTES = X2_HALF * 128;      // this CTA's rows of B for one accumulator
-constexpr uint32_t X2_SF_COL = 2 * X2_BN;
 constexpr int X2_THREADS = 320;
 
-template <int FMT, int NT>
+// BN: columns of an accumulator, 192 or 256. NT: accumulators of a tile.
+template <int FMT, int NT, int BN>
 struct X2 {
     static constexpr int kTiles = Xm<FMT>::kTiles;
+    static constexpr int kAccs = BN == 192 ? 2 : 1;                  // accumulators in tensor memory
+    static constexpr int kHalf = BN / 2, kBBytes = kHalf * 128;      // this CTA's rows of B for one accumulator
+    static constexpr uint32_t kSfCol = kAccs * BN;                   // the scales' first column
     static constexpr int kBTiles = NT + 1;                           // of 128 rows, that hold the tile's columns
     static constexpr int kSfBytes = (1 + kBTiles) * kTiles * 512;
-    static constexpr int kStageBytes = XM_OP_BYTES + NT * X2_B_BYTES + kSfBytes;
+    static constexpr int kStageBytes = XM_OP_BYTES + NT * kBBytes + kSfBytes;
     static constexpr int kSetCols = 4 * kTiles * (1 + kBTiles);      // a step's scales in tensor memory
-    static constexpr int kSets = 128 / kSetCols < 4 ? 128 / kSetCols : 4;
+    static constexpr int kSets = (512 - kSfCol) / kSetCols < 4 ? (512 - kSfCol) / kSetCols : 4;
+    static_assert(NT <= kAccs, "a tile's accumulators are held at once");
     static constexpr int kStages = (227 * 1024 - 1280) / kStageBytes;
     static constexpr size_t kSmem = 1280 + (size_t)kStages * kStageBytes;  // 256 bytes of barriers past the ring
     static_assert((3 * kStages + 4 + 4 + 1) * 8 <= 256, "barriers and the tensor-memory address");
@@ -531,16 +534,17 @@ LYTH_D void x2_commit(uint32_t bar) {  // on this barrier in both CTAs
         : "memory");
 }
 
-template <int FMT, int TY, int NT>
+template <int FMT, int TY, int NT, int BN>
 __global__ void __launch_bounds__(X2_THREADS, 1)
     mx_mma2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                    typename MxElem<TY>::type *C, XmArgs p) {
-    using L = X2<FMT, NT>;
+    using L = X2<FMT, NT, BN>;
     constexpr int T = L::kTiles, S = L::kStages, kSets = L::kSets, NB = L::kBTiles;
+    constexpr bool kTurns = NT < L::kAccs;  // tiles take the accumulators in turn
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * NT * X2_B_BYTES, *sSB = sSA + S * T * 512;
+    uint8_t *sA = smem, *sB = sA + S * XM_OP_BYTES, *sSA = sB + S * NT * L::kBBytes, *sSB = sSA + S * T * 512;
     uint64_t *bars = reinterpret_cast<uint64_t *>(sSB + S * NB * T * 512);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 4 + 4);
     auto full = [&](int s) { return smem_u32(bars + s); };
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
 
     const int warp = (int)warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t crank = blockIdx.x & 1, pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;  // clusters of 2 along x
-    const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + NT * X2_BN - 1) / (NT * X2_BN), ntiles = tiles_m * tiles_n;
+    const uint64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + NT * BN - 1) / (NT * BN), ntiles = tiles_m * tiles_n;
     const uint32_t steps = (p.row_bytes + 127) / 128;
 
     grid_next();
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
         const uint32_t lead = warp_uniform(mapa_shared(full(0), 0));  // the leader's `full` barriers
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs) {
             const uint32_t tm = (uint32_t)(tile % tiles_m), tn = (uint32_t)(tile / tiles_m);
-            const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * (NT * X2_BN));
+            const int m0 = (int)(tm * 256 + 128 * crank), n0 = (int)(tn * (NT * BN));
             for (uint32_t kb = 0; kb < steps; kb++) {
                 if (!xm_wait(empty(stage), phase ^ 1)) { ok = false; break; }
                 const uint32_t lf = lead + 8 * stage;
@@ -601,12 +605,12 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                     mbar_expect_tx(sfull(stage), L::kSfBytes);
                     xm_tma3(smem_u32(sSA + stage * T * 512), &tmSA, 0, (int)(kb * T), m0 >> 7, sfull(stage));
                     xm_tma3(smem_u32(sSB + stage * NB * T * 512), &tmSB, 0, (int)(kb * T), n0 >> 7, sfull(stage));
-                    mbar_expect_tx_cluster(lf, XM_OP_BYTES + NT * X2_B_BYTES);
+                    mbar_expect_tx_cluster(lf, XM_OP_BYTES + NT * L::kBBytes);
                     x2_tma2(smem_u32(sA + stage * XM_OP_BYTES), &tmA, (int)(kb * 128), m0, lf);
 #pragma unroll
                     for (int h = 0; h < NT; h++)
-                        x2_tma2(smem_u32(sB + (stage * NT + h) * X2_B_BYTES), &tmB, (int)(kb * 128),
-                                n0 + h * X2_BN + X2_HALF * (int)crank, lf);
+                        x2_tma2(smem_u32(sB + (stage * NT + h) * L::kBBytes), &tmB, (int)(kb * 128),
+                                n0 + h * BN + L::kHalf * (int)crank, lf);
                 }
                 __syncwarp();
                 if (++stage == S) { stage = 0; phase ^= 1; }
@@ -625,15 +629,15 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
             bool ok = true;
             for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
                 // one accumulator a tile, in turn; or both
-                const uint32_t ab = NT == 1 ? local & 1 : 0u, aphase = NT == 1 ? (local >> 1) & 1 : local & 1;
-                const uint32_t shift = NT == 1 ? ((uint32_t)(tile / tiles_m) & 1) * 2 : 0u;  // 192 tn is 64 mod 128
+                const uint32_t ab = kTurns ? local & 1 : 0u, aphase = kTurns ? (local >> 1) & 1 : local & 1;
+                const uint32_t shift = kTurns ? ((uint32_t)(tile / tiles_m) & 1) * 2 : 0u;  // 192 tn is 64 mod 128
                 for (uint32_t kb = 0; kb < steps; kb++) {
                     if (!xm_wait(full(stage), phase) || !xm_wait(sready(set), sphase)) { ok = false; break; }
                     const uint32_t left = p.row_bytes - kb * 128;
                     const int mmas = left < 128 ? (int)(left / 32) : 4;
-                    const uint32_t sfa = tmem_base + X2_SF_COL + set * L::kSetCols, sfb = sfa + 4 * T + shift;
+                    const uint32_t sfa = tmem_base + L::kSfCol + set * L::kSetCols, sfb = sfa + 4 * T + shift;
                     const uint64_t a = xm_desc_op(smem_u32(sA + stage * XM_OP_BYTES));
-                    const uint64_t b = xm_desc_op(smem_u32(sB + stage * NT * X2_B_BYTES));
+                    const uint64_t b = xm_desc_op(smem_u32(sB + stage * NT * L::kBBytes));
 #pragma unroll
                     for (int h = 0; h < NT; h++) {
                         if (kb == 0 && !xm_wait(tempty(ab + h), aphase ^ 1)) { ok = false; break; }
@@ -642,8 +646,8 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
                                 if (j < mmas)  // columns 192 h on: six words of scales
-                                    x2_mma<FMT>(tmem_base + (ab + h) * X2_BN, a + 2 * j, b + h * (X2_B_BYTES / 16) + 2 * j,
-                                                xm_idesc<FMT>(X2_BN, 256, j), sfa + 4 * (j * T / 4),
+                                    x2_mma<FMT>(tmem_base + (ab + h) * BN, a + 2 * j, b + h * (L::kBBytes / 16) + 2 * j,
+                                                xm_idesc<FMT>(BN, 256, j), sfa + 4 * (j * T / 4),
                                                 sfb + 4 * NB * (j * T / 4) + 6 * h, (kb | (uint32_t)j) != 0);
                             }
                             if (h == NT - 1) x2_commit(empty(stage));
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                     step++;
                 }
                 xm_fence_after();
-                const uint32_t at = tmem_base + ((quad * 32) << 16) + X2_SF_COL + set * L::kSetCols;
+                const uint32_t at = tmem_base + ((quad * 32) << 16) + L::kSfCol + set * L::kSetCols;
 #pragma unroll
                 for (int t = 0; t < T; t++) {
                     x1_st4(at + 4 * t, sa[t]);
@@ -712,18 +716,18 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
         uint32_t local = 0;
         bool ok = true;
         for (uint64_t tile = pair; tile < ntiles && ok; tile += npairs, local++) {
-            const uint64_t row0 = tile % tiles_m * 256 + 128 * crank + quad * 32, n0 = tile / tiles_m * (NT * X2_BN);
+            const uint64_t row0 = tile % tiles_m * 256 + 128 * crank + quad * 32, n0 = tile / tiles_m * (NT * BN);
 #pragma unroll 1
             for (uint32_t h = 0; h < NT; h++) {
-                const uint32_t ab = NT == 1 ? local & 1 : h, aphase = NT == 1 ? (local >> 1) & 1 : local & 1;
+                const uint32_t ab = kTurns ? local & 1 : h, aphase = kTurns ? (local >> 1) & 1 : local & 1;
                 if (!xm_wait(tfull(ab), aphase)) { ok = false; break; }
                 xm_fence_after();
                 XmRow held;
 #pragma unroll 1
-                for (int c = 0; c < X2_BN / 32; c++) {
+                for (int c = 0; c < BN / 32; c++) {
                     uint32_t r[32];
-                    xm_ld32(tmem_base + ab * X2_BN + ((quad * 32) << 16) + c * 32, r);
-                    xm_store32<TY>(C, row0, n0 + h * X2_BN + c * 32, p, held, c + 1 == X2_BN / 32, r);
+                    xm_ld32(tmem_base + ab * BN + ((quad * 32) << 16) + c * 32, r);
+                    xm_store32<TY>(C, row0, n0 + h * BN + c * 32, p, held, c + 1 == BN / 32, r);
                     __syncwarp();
                 }
                 xm_fence_before();
@@ -769,12 +773,12 @@ static bool xm_map_sf(CUtensorMap *map, const void *base, uint64_t words, uint64
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int FMT, int TY, int NT>
+template <int FMT, int TY, int NT, int BN>
 static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &p, cudaStream_t s) {
-    using L = X2<FMT, NT>;
+    using L = X2<FMT, NT, BN>;
     constexpr int T = L::kTiles;
     CUtensorMap ta, tb, tsa, tsb;
-    if (!xm_map(&ta, a, p.row_bytes, p.m, 128) || !xm_map(&tb, b, p.row_bytes, p.n, X2_HALF) ||
+    if (!xm_map(&ta, a, p.row_bytes, p.m, 128) || !xm_map(&tb, b, p.row_bytes, p.n, L::kHalf) ||
         !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, L::kBTiles))
         return LYTH_E_UNSUPPORTED;
     static int fit_of[64] = {0};  // pairs resident at once, asked once per device
@@ -783,7 +787,7 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     if (e != cudaSuccess) return status_of(e);
     int pairs = device_sms() / 2;
     if (dev < 0 || dev >= 64 || fit_of[dev] == 0) {
-        e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
+        e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY, NT, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
         if (e != cudaSuccess) return status_of(e);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -797,16 +801,16 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
         cfg.numAttrs = 1;
         cfg.gridDim = dim3(2u * (unsigned)pairs);
         int fit = 0;
-        if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY, NT>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
+        if (cudaOccupancyMaxActiveClusters(&fit, mx_mma2_kernel<FMT, TY, NT, BN>, &cfg) != cudaSuccess || fit < 1) fit = pairs;
         cudaGetLastError();
         if (fit < pairs) pairs = fit;
         if (dev >= 0 && dev < 64) fit_of[dev] = pairs;
     } else {
         pairs = fit_of[dev];
     }
-    const uint64_t tiles = (p.m + 255) / 256 * ((p.n + NT * X2_BN - 1) / (NT * X2_BN));
+    const uint64_t tiles = (p.m + 255) / 256 * ((p.n + NT * BN - 1) / (NT * BN));
     if ((uint64_t)pairs > tiles) pairs = (int)tiles;
-    return mx_launch(mx_mma2_kernel<FMT, TY, NT>, 2u * (unsigned)pairs, X2_THREADS, L::kSmem, s, 2, ta, tb, tsa, tsb,
+    return mx_launch(mx_mma2_kernel<FMT, TY, NT, BN>, 2u * (unsigned)pairs, X2_THREADS, L::kSmem, s, 2, ta, tb, tsa, tsb,
                                static_cast<typename MxElem<TY>::type *>(c), p);
 }
 
@@ -875,17 +879,26 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     // one tile per SM at most: single SMs, else pairs
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
     if (tiles > (uint64_t)device_sms()) {
-        // Rounds of all pairs over the tiles: of 192 columns, or of 384, whose round is twice the work in 0.85
-        // (NVFP4; 0.9 of the others) of twice the time. 4096 x 14336 x 4096 NVFP4: 17 rounds against 9,
-        // 116 and 106 us; 8192 x 4096 x 14336 MXFP8: 10 against 5, 435 and 358; 4096^3 MXFP4: 5 against 3,
-        // 35.6 and 38.5; 2048 x 4096 x 4096 MXFP8: 3 against 2, 34 and 41.
+        // The tiles' width by the rounds that all pairs make over them: of 192, 256 or 384 columns, a column
+        // of the wider ones taking 0.9 and 0.85 (NVFP4; 0.93 and 0.9 of the others) of one of the first, since
+        // less is staged for the same work. With up to 128 rows of A the weights in flight count, 0.79 of 384.
+        // us for 192, 256, 384: 4096 x 14336 x 4096 NVFP4 117, 107, 105 (17, 13, 9 rounds); 1024 x 4096 x 4096
+        // 16.0, 11.4, 15.1 (2, 1, 1); 4096^3 MXFP4 33.0, 33.0, 36.5 (5, 4, 3); 2048 x 4096 x 4096 MXFP8 32.7,
+        // 29.5, 39.6 (3, 2, 2); 16 x 128256 x 4096 MXFP8 152, 134, 120 (10, 7, 5).
         const uint64_t pairs = (uint64_t)device_sms() / 2, rows = ((uint64_t)m + 255) / 256;
-        const uint64_t one = (rows * (((uint64_t)n + X2_BN - 1) / X2_BN) + pairs - 1) / pairs;
-        const uint64_t two = (rows * (((uint64_t)n + 2 * X2_BN - 1) / (2 * X2_BN)) + pairs - 1) / pairs;
-        if (20 * one > 2 * two * (fmt == LYTH_MX_NVFP4 ? 17 : 18)) {
-            LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 2>(a, b, c, p, s)));
+        const bool nv = fmt == LYTH_MX_NVFP4;
+        auto cost = [&](uint64_t width, uint64_t column) {
+            return (rows * ((n + width - 1) / width) + pairs - 1) / pairs * width * column;
+        };
+        const uint64_t c192 = cost(192, 200), c256 = cost(256, nv ? 179 : 186);
+        const uint64_t c384 = cost(384, m <= 128 ? 158 : nv ? 170 : 181);
+        if (c256 < c192 && c256 < c384) {
+            LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 1, 256>(a, b, c, p, s)));
         }
-        LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 1>(a, b, c, p, s)));
+        if (c384 < c192) {
+            LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 2, 192>(a, b, c, p, s)));
+        }
+        LYTH_MX_DISPATCH(fmt, ty, return (x2_launch<FMT, TY, 1, 192>(a, b, c, p, s)));
     }
     LYTH_MX_DISPATCH(fmt, ty, return (x1_launch<FMT, TY>(a, b, c, p, s)));
     return LYTH_E_UNSUPPORTED;

@@ -676,3 +676,12 @@ def test_a_chain_of_dependent_calls(cuda, rows):
         torch.cuda.synchronize()
         lb.dequantize_mx(lb.MX_FP8, *again, out)
         assert torch.equal(codes, again[0]) and torch.equal(got, out)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,n,k", [(1, 19500, 192), (100, 19001, 64), (128, 19500, 1024), (129, 19456, 320), (600, 14336, 128),
+                                   (250, 14336, 320), (1000, 4100, 1000), (512, 14330, 640), (2048, 4096, 192)])
+def test_matmul_tile_widths(cuda, fmt, m, n, k):
+    # more 128 x 128 tiles than SMs: each width of a pair's tile, in one round and in several, rows and
+    # columns of it that do not exist
+    test_matmul(cuda, fmt, torch.bfloat16, m, n, k)
