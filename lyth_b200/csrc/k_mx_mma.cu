@@ -102,7 +102,7 @@ struct XmArgs {
     uint32_t row_bytes;      // bytes of a row of codes
     uint32_t words;          // scale tiles along k
     float alpha;
-    bool vec;                // rows of C start on 32 bytes
+    bool vec, vec4;          // rows of C start on 32 bytes; on four elements
 };
 
 // A lane's row of C, stored 32 columns at a time from left to right. Rows that start on 32 bytes are
@@ -441,12 +441,18 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
                 if ((q & (ks - 1)) == ks - 1) {
                     const uint32_t i = i0 + (q >> klog) * X1_THREADS;
                     if (i < items) {
-                        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+                        const float f[4] = {__fmul_rn(p.alpha, sum.x), __fmul_rn(p.alpha, sum.y), __fmul_rn(p.alpha, sum.z),
+                                            __fmul_rn(p.alpha, sum.w)};
                         const uint64_t n0 = (uint64_t)tn * XM_BN + rank * width + (i & ((1u << glog) - 1)) * 4;
                         typename MxElem<TY>::type *to = C + ((uint64_t)tm * XM_BM + (i >> glog)) * p.ldc + n0;
+                        if (p.vec4 && n0 + 4 <= p.n) {
+                            if constexpr (TY == 0) *reinterpret_cast<float4 *>(to) = make_float4(f[0], f[1], f[2], f[3]);
+                            else *reinterpret_cast<uint2 *>(to) = make_uint2(mx_pack2<TY>(f[0], f[1]), mx_pack2<TY>(f[2], f[3]));
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (n0 + j < p.n) to[j] = MxElem<TY>::round(__fmul_rn(p.alpha, f[j]));
+                            for (int j = 0; j < 4; j++)
+                                if (n0 + j < p.n) to[j] = MxElem<TY>::round(f[j]);
+                        }
                     }
                     sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
@@ -876,6 +882,7 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     p.words = (uint32_t)(k / (4 * mx_block(fmt)));
     p.alpha = alpha;
     p.vec = aligned32(c) && ldc * mx_ty_bytes(ty) % 32 == 0;
+    p.vec4 = ((uintptr_t)c & (4 * mx_ty_bytes(ty) - 1)) == 0 && ldc % 4 == 0;
     // one tile per SM at most: single SMs, else pairs
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
     if (tiles > (uint64_t)device_sms()) {
