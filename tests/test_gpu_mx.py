@@ -685,3 +685,55 @@ def test_matmul_tile_widths(cuda, fmt, m, n, k):
     # more 128 x 128 tiles than SMs: each width of a pair's tile, in one round and in several, rows and
     # columns of it that do not exist
     test_matmul(cuda, fmt, torch.bfloat16, m, n, k)
+
+
+def test_inputs_written_on_another_stream(cuda):
+    # an event of another stream between two calls of this one, eager and captured
+    fmt, n, k = lb.MX_FP4, 8192, 4096
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(40, k, generator=gen).bfloat16().to(cuda)
+    ws = [torch.randn(n, k, generator=gen).bfloat16().to(cuda) for _ in range(3)]
+    one = torch.ones(k, dtype=torch.bfloat16, device=cuda)
+    a, w = empty(fmt, 40, k, cuda), empty(fmt, n, k, cuda)
+    c, y = torch.empty(40, n, dtype=torch.bfloat16, device=cuda), torch.empty(4, n, dtype=torch.bfloat16, device=cuda)
+    side, src = torch.cuda.Stream(), torch.empty_like(ws[0])
+
+    def step():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            lb.quantize_mx(fmt, src, *w)
+        lb.rmsnorm_mx(fmt, x, one, *a)
+        torch.cuda.current_stream().wait_stream(side)
+        lb.gemv_mx(fmt, x[:4], *w, y)
+        lb.matmul_mx(fmt, *a, *w, c)
+
+    want = []
+    for t in ws:
+        src.copy_(t)
+        torch.cuda.synchronize()
+        lb.quantize_mx(fmt, src, *w)
+        lb.rmsnorm_mx(fmt, x, one, *a)
+        torch.cuda.synchronize()
+        lb.gemv_mx(fmt, x[:4], *w, y)
+        torch.cuda.synchronize()
+        lb.matmul_mx(fmt, *a, *w, c)
+        torch.cuda.synchronize()
+        want.append((c.clone(), y.clone()))
+    main = torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        for i in range(30):
+            src.copy_(ws[i % 3])
+            step()
+            got = c.clone(), y.clone()
+            main.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, want[i % 3])), i
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=main):
+            step()
+        for i in range(30):
+            src.copy_(ws[i % 3])
+            g.replay()
+            main.synchronize()
+            assert torch.equal(c, want[i % 3][0]) and torch.equal(y, want[i % 3][1]), i
+    torch.cuda.synchronize()
