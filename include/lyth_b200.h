@@ -558,7 +558,7 @@ int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, 
  * m <= LYTH_GEMV_MX_MAX_M, w n x cols in `fmt`; f32 accumulation, y rounded once to `ty`. A row of y
  * does not depend on what the other rows of x hold. bf16 x is brought into f16's range by 128 columns
  * (E4M3 weights: 64) of a row at a time, by a power of two: values below 2^-31 of the largest among
- * them lose bits, all others are exact. */
+ * them lose bits; all other products are exact before the f32 sums, whatever the block scales. */
 #define LYTH_GEMV_MX_MAX_M 8
 int lyth_b200_gemv_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, const void *x, uint64_t ldx,
                       const uint8_t *w, const uint8_t *w_scales, float alpha, void *y, uint64_t ldy,

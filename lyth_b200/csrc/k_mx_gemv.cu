@@ -33,7 +33,12 @@
 // Range: bf16 x is brought into f16 by a power of two for each step's columns (128, of E4M3 weights 64
 // neighbouring values of a token; their largest exponent to 2^14) and taken back in f32. Of those values,
 // ones below 2^-31 of the largest lose bits (eight bits end at f16's 2^-24); every other product is exact
-// before the f32 sums.
+// before the f32 sums. A step's sum is below 2^28 and a multiple of 2^-33. E8M0 scales reach 2^-127 and
+// 2^127, so the sum times the scale could leave f32 where the product does not: the power of two that
+// takes x back comes in two factors, 2^-30 .. 2^30 of it before the scale and the rest after, and then
+// neither end is passed before the product passes it (one token through 14336 x 4096 MXFP8 13.2 us with one
+// factor and with two, eight 25.4 and 26.6; four through 4096 x 14336 MXFP4 17.4 and 18.4). NVFP4's scales
+// end at 448 and 2^-9: one factor does.
 #include "mbar.cuh"
 #include "mx.cuh"
 
@@ -46,6 +51,9 @@ constexpr int XV_TEAM = XV_WARPS / 2;               // a team takes every other 
 constexpr uint32_t XV_STAGES = 4;                   // of the ring: even, since a team owns every other one
 constexpr int XV_PRODUCERS = 4;                     // warps, one per quad of a group
 constexpr int XV_THREADS = 32 * (XV_WARPS + XV_PRODUCERS);
+// f32 factors per token and step that take bf16 x back: two of E8M0 formats (see above), f16 x none.
+template <int FMT, int TY>
+constexpr uint32_t kXvBack = TY != LYTH_NARROW_BF16 ? 0 : FMT == LYTH_MX_NVFP4 ? 1 : 2;
 // Groups whose partial sums are kept before they are added up: all of a block's, up to this many.
 template <int PAIRS>
 constexpr int kXvBatch = PAIRS == 4 ? 4 : 8;
@@ -214,15 +222,28 @@ LYTH_D void xv_steps(const uint8_t *at, uint32_t pitch, uint32_t it, uint32_t x_
 #pragma unroll
         for (int pr = 0; pr < PAIRS; pr++) {
             if constexpr (TY == LYTH_NARROW_BF16) {  // the step's sum, then back from x's f16 range
-                float d0 = 0.0f, d1 = 0.0f;
+                float d0 = 0.0f, d1 = 0.0f, xs;
+                float2 c0[kSub], c1[kSub];
 #pragma unroll
                 for (int k = 0; k < kSub; k++) {
-                    d0 = __fmaf_rn(cc[s][pr][k][0], f0[k].x, d0);
-                    d1 = __fmaf_rn(cc[s][pr][k][2], f1[k].x, d1);
-                    d0 = __fmaf_rn(cc[s][pr][k][1], f0[k].y, d0);
-                    d1 = __fmaf_rn(cc[s][pr][k][3], f1[k].y, d1);
+                    c0[k] = make_float2(cc[s][pr][k][0], cc[s][pr][k][1]);
+                    c1[k] = make_float2(cc[s][pr][k][2], cc[s][pr][k][3]);
                 }
-                const float xs = xs_at[pr][x_step + s * XV_TEAM];
+                if constexpr (kXvBack<FMT, TY> == 2) {
+                    const float2 back = reinterpret_cast<const float2 *>(xs_at[pr])[x_step + s * XV_TEAM];
+                    c0[0] = mx_mul2(c0[0], make_float2(back.x, back.x));
+                    c1[0] = mx_mul2(c1[0], make_float2(back.x, back.x));
+                    xs = back.y;
+                } else {
+                    xs = xs_at[pr][x_step + s * XV_TEAM];
+                }
+#pragma unroll
+                for (int k = 0; k < kSub; k++) {
+                    d0 = __fmaf_rn(c0[k].x, f0[k].x, d0);
+                    d1 = __fmaf_rn(c1[k].x, f1[k].x, d1);
+                    d0 = __fmaf_rn(c0[k].y, f0[k].y, d0);
+                    d1 = __fmaf_rn(c1[k].y, f1[k].y, d1);
+                }
                 acc[pr][0] = __fmaf_rn(d0, xs, acc[pr][0]);
                 acc[pr][1] = __fmaf_rn(d1, xs, acc[pr][1]);
             } else {
@@ -253,8 +274,12 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
     const uint32_t xunits = p.xsteps * 4 * kUnits;        // 16-byte units of x per token
     const uint32_t pitch = p.seg + 64;                    // of rows in a stage: eight read at once hit all banks
     uint4 *sx = reinterpret_cast<uint4 *>(sm + XV_STAGES * p.stage_bytes);
-    float *s_scale = reinterpret_cast<float *>(sx + p.m * (xunits + 4));  // of bf16 x: [token][step]
-    float *s_part = s_scale + (TY == LYTH_NARROW_BF16 ? p.m * p.xsteps : 0);  // [group][warp][token][row]
+    constexpr uint32_t kBack = kXvBack<FMT, TY>;
+    // of bf16 x: [token][step][factor]; of two factors an odd number of pairs, so that two tokens' lie in
+    // different banks
+    const uint32_t bpitch = kBack == 2 ? (p.xsteps | 1) * 2 : p.xsteps * kBack;
+    float *s_scale = reinterpret_cast<float *>(sx + p.m * (xunits + 4));
+    float *s_part = s_scale + p.m * bpitch;               // [group][warp][token][row]
     auto full = [&](uint32_t s) { return smem_u32(bars + s); };
     auto empty = [&](uint32_t s) { return smem_u32(bars + XV_STAGES + s); };
     const uint32_t xbar = smem_u32(bars + 2 * XV_STAGES); // the consumers' meeting point
@@ -332,7 +357,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             x_at[pr] = smem_u32(sx + min(2u * pr + (g >> 2), p.m - 1) * (xunits + 4) + t);
         const float *xs_at[PAIRS];  // of this lane's columns' token
 #pragma unroll
-        for (int pr = 0; pr < PAIRS; pr++) xs_at[pr] = s_scale + min(2u * pr + (t >> 1), p.m - 1) * p.xsteps;
+        for (int pr = 0; pr < PAIRS; pr++) xs_at[pr] = s_scale + min(2u * pr + (t >> 1), p.m - 1) * bpitch;
         const T *x = static_cast<const T *>(p.x);
         uint32_t stage = 0, phase = 0;
         bool ok = true, staged = false;
@@ -374,11 +399,16 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
                                 uint32_t top = xv_top(v[h]);
 #pragma unroll
                                 for (int o = 1; o < 4 * kUnits; o *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                                // 2^(14 - e), e the largest exponent; it and its inverse are normal f32 numbers
+                                // 2^(14 - e), e the largest exponent; it and its inverse, whole or in two
+                                // factors, are normal f32 numbers
                                 const int sh = min(14 - ((int)top - 127), 126);
                                 v[h] = xv_f16(v[h], __uint_as_float((uint32_t)(127 + sh) << 23));
-                                if (in && u[h] % (4 * kUnits) == 0)
-                                    s_scale[tok[h] * p.xsteps + owner / 4] = __uint_as_float((uint32_t)(127 - sh) << 23);
+                                const int near = kBack == 2 ? max(-30, min(30, -sh)) : 0;
+                                float *back = s_scale + tok[h] * bpitch + owner / 4 * kBack;
+                                if (in && u[h] % (4 * kUnits) == 0) {
+                                    if constexpr (kBack == 2) *back++ = __uint_as_float((uint32_t)(127 + near) << 23);
+                                    *back = __uint_as_float((uint32_t)(127 - sh - near) << 23);
+                                }
                             }
                             if (in) sx[tok[h] * (xunits + 4) + owner / 4 * (4 * kUnits) + u[h] % kUnits * 4 + owner % 4] = v[h];
                         }
@@ -451,9 +481,9 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
     // tokens x 1024 E2M1 bytes are 32 KiB).
     const uint32_t groups = (p.quads_each + (p.quads_more ? 1 : 0) + 3) / 4;
     const size_t sums = (size_t)(groups < (uint32_t)kXvBatch<PAIRS> ? groups : kXvBatch<PAIRS>) * XV_WARPS * 2 * PAIRS * 16 * sizeof(float);
-    const size_t step_x = (size_t)p.m * ((FMT == LYTH_MX_FP8 ? 8 : 16) * 16 + (TY == LYTH_NARROW_BF16 ? 4 : 0));
+    const size_t step_x = (size_t)p.m * ((FMT == LYTH_MX_FP8 ? 8 : 16) * 16 + kXvBack<FMT, TY> * sizeof(float));
     const uint32_t steps = (p.row_bytes + 63) / 64;
-    const size_t room = 226 * 1024 - sums - p.m * 64;
+    const size_t pads = p.m * (64 + (kXvBack<FMT, TY> == 2 ? 8 : 0)), room = 226 * 1024 - sums - pads;
     auto ring = [&](uint32_t seg) {
         p.seg = seg;
         p.segs = (p.row_bytes + seg - 1) / seg;
@@ -466,7 +496,7 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
     if (held + steps * step_x > room) held = ring(1024);
     p.chunk = held + steps * step_x <= room ? p.segs : (uint32_t)((room - held) / (p.seg / 64 * step_x));
     p.xsteps = p.chunk == p.segs ? steps : p.chunk * (p.seg / 64);
-    const size_t smem = held + p.xsteps * step_x + p.m * 64 + sums;
+    const size_t smem = held + p.xsteps * step_x + pads + sums;
     static bool set[64] = {false};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
