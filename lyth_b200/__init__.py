@@ -383,16 +383,25 @@ def gemv_dequant(fmt: int, w, scales, out, group: int = 64, stream=None) -> None
 # ----------------------------------------------------------------------------- block-scaled formats
 MX_FP8, MX_FP4, MX_NVFP4 = 0, 1, 2
 GEMV_MX_MAX_M = 8
+_U32_MAX = (1 << 32) - 1
+
+
+def _mx_fits(what, cols, rows=0):
+    """Refuses what the ABI's integers do not hold: ctypes would cut it to their width without a word."""
+    if not (0 <= cols <= _U32_MAX and 0 <= rows <= 1 << 40):
+        raise LythError(E_INVALID, f"{what}: {rows} x {cols}" if rows else f"{what}: {cols} columns")
 
 
 def mx_row_bytes(fmt: int, cols: int) -> int:
-    """Bytes of one row of codes: cols rounded up to four blocks, 8 or 4 bits each."""
-    return int(lib.lyth_b200_mx_row_bytes(fmt, cols))
+    """Bytes of one row of codes: cols rounded up to four blocks, 8 or 4 bits each. 0 of an unknown format."""
+    _mx_fits("mx_row_bytes", cols)
+    return int(lib.lyth_b200_mx_row_bytes(fmt, cols)) if fmt in _MX_WORD else 0
 
 
 def mx_scale_bytes(fmt: int, rows: int, cols: int) -> int:
-    """Bytes of the tiled scales of a rows x cols matrix."""
-    return int(lib.lyth_b200_mx_scale_bytes(fmt, rows, cols))
+    """Bytes of the tiled scales of a rows x cols matrix. 0 of an unknown format."""
+    _mx_fits("mx_scale_bytes", cols, rows)
+    return int(lib.lyth_b200_mx_scale_bytes(fmt, rows, cols)) if fmt in _MX_WORD else 0
 
 
 def mx_empty(fmt: int, rows: int, cols: int, device):
@@ -457,6 +466,8 @@ def _mx_rows(t, name, dev, dtype=None):
         rows, cols = t.shape
     except ValueError:
         raise ValueError(f"{name}: expected two dimensions, got {t.dim()}") from None
+    if cols > _U32_MAX:
+        _mx_fits(name, cols)
     ld, inner = t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name}: rows must be contiguous")
@@ -544,6 +555,8 @@ def matmul_mx(fmt: int, a, a_scales, b, b_scales, c, alpha: float = 1.0, stream=
     if a.dim() != 2:
         raise ValueError(f"a: expected two dimensions, got {a.dim()}")
     cols = a.shape[1] << (fmt != MX_FP8)
+    if m > _U32_MAX or cols > _U32_MAX:
+        raise LythError(E_INVALID, f"matmul_mx: {m} x {n} x {cols}")
     ap, asp = _mx_operand(fmt, m, cols, a, a_scales, dev, "a")
     bp, bsp = _mx_operand(fmt, n, cols, b, b_scales, dev, "b")
     check(lib.lyth_b200_matmul_mx(fmt, _mx_ty(c, "c"), m, n, cols, ap, asp, bp, bsp, alpha, cp, ldc, _mx_stream(stream, dev)),
@@ -558,6 +571,8 @@ def gemv_mx(fmt: int, x, w, w_scales, y, alpha: float = 1.0, stream=None) -> Non
     m2, n, yp, ldy = _mx_rows(y, "y", dev, x.dtype)
     if m2 != m:
         raise ValueError(f"gemv shapes {tuple(x.shape)} -> {tuple(y.shape)}")
+    if m > GEMV_MX_MAX_M:
+        raise LythError(E_UNSUPPORTED, f"gemv_mx: {m} rows of x, {GEMV_MX_MAX_M} at most")
     wp, wsp = _mx_operand(fmt, n, cols, w, w_scales, dev, "w")
     check(lib.lyth_b200_gemv_mx(fmt, _mx_ty(x, "x"), m, n, cols, xp, ldx, wp, wsp, alpha, yp, ldy, _mx_stream(stream, dev)),
           "gemv_mx")

@@ -225,3 +225,69 @@ def test_wrappers_pass_no_rows_through(on_device0):
         lb.quantize_mx(fmt, Fake((0, 64), torch.bfloat16), *held(fmt, 0, 64))
         lb.matmul_mx(fmt, *held(fmt, 0, 64), *held(fmt, 8, 64), Fake((0, 8), torch.float32))
         lb.gemv_mx(fmt, Fake((0, 64), torch.float16), *held(fmt, 8, 64), Fake((0, 8), torch.float16))
+
+
+# ------------------------------------------------------------------ sizes that a 32-bit argument would cut
+WIDE = (1 << 32) + 64
+
+
+def refused(call, *args, **kw):
+    with pytest.raises(lb.LythError) as e:
+        call(*args, **kw)
+    assert e.value.status == lb.E_INVALID
+
+
+def wide_held(fmt, rows, cols):
+    import torch
+
+    k = mx.padded(fmt, cols)
+    return (Fake((rows, k if fmt == lb.MX_FP8 else k // 2), torch.uint8), Fake((-(-rows // 128) * 128 * k // mx.BLOCK[fmt],), torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("cols", [WIDE, (1 << 32), (1 << 30) + 1, (1 << 33) + 1])
+def test_wrappers_refuse_columns_past_the_limit(on_device0, fmt, cols):
+    # no rows: a size that arrived cut would be taken as nothing to do
+    import torch
+
+    bf = torch.bfloat16
+    x, ops = Fake((0, cols), bf), wide_held(fmt, 0, cols)
+    refused(lb.quantize_mx, fmt, x, *ops)
+    refused(lb.dequantize_mx, fmt, *ops, x)
+    refused(lb.rmsnorm_mx, fmt, x, Fake((cols,), bf), *ops)
+    refused(lb.matmul_mx, fmt, *ops, *wide_held(fmt, 4, cols), Fake((0, 4), bf))
+    refused(lb.gemv_mx, fmt, x, *wide_held(fmt, 4, cols), Fake((0, 4), bf))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_wrappers_refuse_rows_past_the_limit(on_device0, fmt):
+    import torch
+
+    bf = torch.bfloat16
+    k = 128
+    # 2^32 rows cut to 32 bits are none, which would be nothing to do
+    refused(lb.matmul_mx, fmt, *wide_held(fmt, 1 << 32, k), *wide_held(fmt, 4, k), Fake((1 << 32, 4), bf))
+    refused(lb.matmul_mx, fmt, *wide_held(fmt, 4, k), *wide_held(fmt, 1 << 32, k), Fake((4, 1 << 32), bf))
+    refused(lb.gemv_mx, fmt, Fake((1, k), bf), *wide_held(fmt, 1 << 32, k), Fake((1, 1 << 32), bf))
+    with pytest.raises(lb.LythError) as e:
+        lb.gemv_mx(fmt, Fake((1 << 32, k), bf), *wide_held(fmt, 4, k), Fake((1 << 32, 4), bf))
+    assert e.value.status == lb.E_UNSUPPORTED  # more rows than GEMV_MX_MAX_M, however many
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_sizes_of_what_no_call_takes(fmt):
+    refused(lb.mx_row_bytes, fmt, WIDE)
+    refused(lb.mx_scale_bytes, fmt, 4, WIDE)
+    refused(lb.mx_empty, fmt, 4, WIDE, "cpu")
+    refused(lb.mx_row_bytes, fmt, -1)
+    refused(lb.mx_scale_bytes, fmt, -1, 64)
+    refused(lb.mx_scale_bytes, fmt, 1 << 64, 64)
+
+
+def test_a_format_past_32_bits_is_unknown(on_device0):
+    import torch
+
+    assert lb.mx_row_bytes(1 << 32, 64) == 0 and lb.mx_scale_bytes(1 << 32, 4, 64) == 0
+    with pytest.raises(lb.LythError) as e:
+        lb.quantize_mx(1 << 32, Fake((0, 64), torch.bfloat16), *held(lb.MX_FP8, 0, 64))
+    assert e.value.status == lb.E_UNSUPPORTED
