@@ -39,6 +39,8 @@
 // neither end is passed before the product passes it (one token through 14336 x 4096 MXFP8 13.2 us with one
 // factor and with two, eight 25.4 and 26.6; four through 4096 x 14336 MXFP4 17.4 and 18.4). NVFP4's scales
 // end at 448 and 2^-9: one factor does.
+#include <atomic>
+
 #include "mbar.cuh"
 #include "mx.cuh"
 
@@ -497,7 +499,7 @@ static int xv_launch(XvArgs p, cudaStream_t s) {
     p.chunk = held + steps * step_x <= room ? p.segs : (uint32_t)((room - held) / (p.seg / 64 * step_x));
     p.xsteps = p.chunk == p.segs ? steps : p.chunk * (p.seg / 64);
     const size_t smem = held + p.xsteps * step_x + pads + sums;
-    static bool set[64] = {false};
+    static std::atomic<bool> set[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);

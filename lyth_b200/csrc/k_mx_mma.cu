@@ -12,6 +12,8 @@
 // stored; k is whole scale words, so the last step's MMAs are only fewer. Every wait is bounded.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "mbar.cuh"
 #include "mx.cuh"
 
@@ -787,12 +789,13 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     if (!xm_map(&ta, a, p.row_bytes, p.m, 128) || !xm_map(&tb, b, p.row_bytes, p.n, L::kHalf) ||
         !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, L::kBTiles))
         return LYTH_E_UNSUPPORTED;
-    static int fit_of[64] = {0};  // pairs resident at once, asked once per device
+    static std::atomic<int> fit_of[64];  // pairs resident at once, asked once per device (0: not yet)
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);
-    int pairs = device_sms() / 2;
-    if (dev < 0 || dev >= 64 || fit_of[dev] == 0) {
+    int pairs = dev >= 0 && dev < 64 ? fit_of[dev].load() : 0;
+    if (pairs == 0) {
+        pairs = device_sms() / 2;
         e = cudaFuncSetAttribute(mx_mma2_kernel<FMT, TY, NT, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem);
         if (e != cudaSuccess) return status_of(e);
         cudaLaunchAttribute attr[1];
@@ -811,8 +814,6 @@ static int x2_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
         cudaGetLastError();
         if (fit < pairs) pairs = fit;
         if (dev >= 0 && dev < 64) fit_of[dev] = pairs;
-    } else {
-        pairs = fit_of[dev];
     }
     const uint64_t tiles = (p.m + 255) / 256 * ((p.n + NT * BN - 1) / (NT * BN));
     if ((uint64_t)pairs > tiles) pairs = (int)tiles;
@@ -828,7 +829,7 @@ static int x1_launch(const uint8_t *a, const uint8_t *b, void *c, const XmArgs &
     if (!xm_map(&ta, a, p.row_bytes, p.m, a_rows) || !xm_map(&tb, b, p.row_bytes, p.n, XM_BN) ||
         !xm_map_sf(&tsa, p.sa, p.words, p.m, T, 1) || !xm_map_sf(&tsb, p.sb, p.words, p.n, T, 1))
         return LYTH_E_UNSUPPORTED;
-    static bool done[64] = {false};
+    static std::atomic<bool> done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return status_of(e);

@@ -173,17 +173,16 @@ typedef CUresult (*PFN_encode_tiled)(CUtensorMap *, CUtensorMapDataType, cuuint3
                                      CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                      CUtensorMapFloatOOBfill);
 
+// Looked up once per process; threads that come first together wait for the one that looks.
 inline PFN_encode_tiled tensor_map_encoder() {
-    static PFN_encode_tiled fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    static const PFN_encode_tiled fn = []() -> PFN_encode_tiled {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_encode_tiled>(p);
-    }
+            return reinterpret_cast<PFN_encode_tiled>(p);
+        return nullptr;
+    }();
     return fn;
 }
 
