@@ -173,8 +173,8 @@ typedef CUresult (*PFN_encode_tiled)(CUtensorMap *, CUtensorMapDataType, cuuint3
                                      CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                                      CUtensorMapFloatOOBfill);
 
-// Looked up once per process; threads that come first together wait for the one that looks.
-inline PFN_encode_tiled tensor_map_encoder() {
+// The driver's entry, looked up once per process; threads that come first together wait for the one that looks.
+inline PFN_encode_tiled tensor_map_lookup() {
     static const PFN_encode_tiled fn = []() -> PFN_encode_tiled {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -185,5 +185,20 @@ inline PFN_encode_tiled tensor_map_encoder() {
     }();
     return fn;
 }
+// It wants a context current on the calling thread. The runtime makes its device's current at a thread's first
+// launch or allocation, which may come after the map: a thread that has none is given it here, and a
+// caller's own context is left alone.
+inline CUresult tensor_map_encode(CUtensorMap *map, CUtensorMapDataType type, cuuint32_t rank, void *base,
+                                  const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                                  const cuuint32_t *step, CUtensorMapInterleave interleave, CUtensorMapSwizzle swizzle,
+                                  CUtensorMapL2promotion l2, CUtensorMapFloatOOBfill fill) {
+    const PFN_encode_tiled fn = tensor_map_lookup();
+    CUresult r = fn(map, type, rank, base, dims, strides, box, step, interleave, swizzle, l2, fill);
+    int dev = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+        r = fn(map, type, rank, base, dims, strides, box, step, interleave, swizzle, l2, fill);
+    return r;
+}
+inline PFN_encode_tiled tensor_map_encoder() { return tensor_map_lookup() ? tensor_map_encode : nullptr; }
 
 }  // namespace lyth

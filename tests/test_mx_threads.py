@@ -105,3 +105,42 @@ def test_products_as_the_first_calls_of_eight_threads(cuda, n):
     r = subprocess.run([sys.executable, "-c", FIRST.replace("WIDTH", str(n))], cwd=ROOT, capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("OK"), r.stdout + r.stderr
+
+
+NO_CONTEXT = """
+import threading
+import torch
+import lyth_b200 as lb
+
+cuda = torch.device("cuda")
+codes, scales = lb.mx_empty(lb.MX_FP8, 128, 512, cuda)
+codes.fill_(0x38), scales.fill_(127)
+c, d = torch.zeros(128, 128, device=cuda), torch.zeros(128, 256, device=cuda)
+a, b = torch.ones(128, 64, dtype=torch.bfloat16, device=cuda), torch.ones(64, 256, dtype=torch.bfloat16, device=cuda)
+torch.cuda.synchronize()
+failed = []
+
+
+def work(call):
+    try:
+        call()
+    except BaseException as e:
+        failed.append(e)
+
+
+for call in (lambda: lb.matmul_mx(lb.MX_FP8, codes, scales, codes, scales, c, stream=0), lambda: lb.matmul_bf16(a, b, d, stream=0)):
+    t = threading.Thread(target=work, args=(call,))
+    t.start()
+    t.join()
+assert not failed, failed
+torch.cuda.synchronize()
+assert bool((c == 512).all()) and bool((d == 64).all())
+print("OK")
+"""
+
+
+@pytest.mark.gpu
+def test_products_on_threads_that_have_no_context(cuda):
+    # a thread whose first CUDA work is the product: the tensor map is made before the runtime has set it up
+    r = subprocess.run([sys.executable, "-c", NO_CONTEXT], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("OK"), r.stdout + r.stderr
