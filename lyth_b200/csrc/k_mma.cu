@@ -148,15 +148,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     if (++stage == MM_STAGES) { stage = 0; phase ^= 1; }
                 }
             }
-            // Normally every load has been consumed by the MMAs before the block-wide sync
-            // below. After a timed-out wait, give the stages this thread may have in flight a
-            // bounded chance to land before the block leaves.
-            if (!ok) {
-                for (int s = 0; s < MM_STAGES; s++) {
-                    mm_wait(full(stage), phase);
-                    if (++stage == MM_STAGES) { stage = 0; phase ^= 1; }
-                }
-            }
+            ring_drain(stage, phase, MM_STAGES, [&](uint32_t s, uint32_t parity) { mm_wait(full(s), parity); });
         }
     } else if (warp == 1) {
         if (lane == 0) {

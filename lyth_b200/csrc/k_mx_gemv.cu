@@ -338,13 +338,7 @@ __global__ void __launch_bounds__(XV_THREADS, 1) mx_gemv_kernel(const __grid_con
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        // Normally every copy has been consumed. After a timed-out wait, give the stages that may be in
-        // flight a bounded chance to land before the block leaves.
-        if (!ok)
-            for (uint32_t s = 0; s < XV_STAGES; s++) {
-                xv_wait(full(stage), phase ^ 1);
-                if (++stage == XV_STAGES) { stage = 0; phase ^= 1; }
-            }
+        ring_drain(stage, phase, XV_STAGES, [&](uint32_t s, uint32_t parity) { xv_wait(full(s), parity); });
     } else {  // ------------------------------------------------------------------------------- consumers
         const uint32_t g = lane >> 2, t = lane & 3;
         // x in shared memory: [token][step][unit][lane of the quad], tokens 64 bytes apart modulo 128, so

@@ -328,14 +328,7 @@ __global__ void __launch_bounds__(X1_THREADS, 1)
             __syncwarp();
             if (++stage == S) { stage = 0; phase ^= 1; }
         }
-        // After a timed-out wait, give the stages that may be in flight a bounded chance to land before
-        // the block leaves.
-        if (!ok) {
-            for (int s = 0; s < S; s++) {
-                xm_wait(full(stage), phase);
-                if (++stage == S) { stage = 0; phase ^= 1; }
-            }
-        }
+        ring_drain(stage, phase, S, [&](uint32_t s, uint32_t parity) { xm_wait(full(s), parity); });
     } else if (warp == 1) {
         uint32_t stage = 0, phase = 0, set = 0, sphase = 0;
         for (uint32_t kb = k0; kb < k1; kb++) {
@@ -624,6 +617,9 @@ __global__ void __launch_bounds__(X2_THREADS, 1)
                 if (++stage == S) { stage = 0; phase ^= 1; }
             }
         }
+        // This CTA's scale copies; its halves of A and B are waited for on the leader's barriers, by the
+        // warp that issues the MMAs.
+        ring_drain(stage, phase, S, [&](uint32_t s, uint32_t parity) { xm_wait(sfull(s), parity); });
         // Tail: every stage released by the MMA's commit, so no arrival is still on its way to this
         // CTA's barriers when it leaves.
         if (ok)

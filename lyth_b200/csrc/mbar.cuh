@@ -76,6 +76,20 @@ LYTH_D bool mbar_wait_warp(uint32_t bar, uint32_t parity, int *err) {
     atomicExch(err, 1);
     return false;
 }
+// What a producer does once it issues no more, because all is issued or because a wait of its own ran out: a
+// bounded wait for the last copy into each stage of its ring, whether or not another role still takes them,
+// so that none is in flight into the block's shared memory when the block leaves. (stage, phase) is where the
+// producer would fill next and the parity of that lap: a stage's last copy is of the lap before, parity
+// phase ^ 1, which a barrier that no copy has used reports as complete.
+#pragma nv_exec_check_disable
+template <class Wait>
+LYTH_HD void ring_drain(uint32_t stage, uint32_t phase, uint32_t stages, Wait wait) {
+#pragma unroll 1
+    for (uint32_t s = 0; s < stages; s++) {
+        wait(stage, phase ^ 1);
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
+}
 // One lane of a converged warp; values every lane holds, told to the compiler as uniform.
 LYTH_D bool elect_one() {
     uint32_t one;
