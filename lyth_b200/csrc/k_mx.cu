@@ -116,6 +116,12 @@ __global__ void __launch_bounds__(kMxThreads)
 #pragma unroll
     for (int u = 0; u < U; u++) {
         uint32_t h[8], o[kMxWords<TY>];
+        const float s = mx_scales2<FMT>(byte[u]).x;
+        if constexpr (FMT == LYTH_MX_NVFP4 && TY != 0) {
+            mx_nvfp4_back<TY>(in[u][0], in[u][1], s, g, o);
+            mx_store<TY, VEC>(out + row[u] * f.ld, c[u], f.cols, row[u] < f.rows, o);
+            continue;
+        }
         if constexpr (FMT == LYTH_MX_FP8) {
 #pragma unroll
             for (int i = 0; i < 4; i++) e4m3x4_f16(in[u][i], h[2 * i], h[2 * i + 1]);
@@ -128,7 +134,6 @@ __global__ void __launch_bounds__(kMxThreads)
                 for (int j = 0; j < 4; j++) h[4 * i + j] = a[j];
             }
         }
-        const float s = mx_scales2<FMT>(byte[u]).x;
         float v[16];
 #pragma unroll
         for (int i = 0; i < 8; i++) {

@@ -413,6 +413,13 @@ LYTH_D float2 mx_mul2(float2 a, float2 b) {
         : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
     return *reinterpret_cast<float2 *>(&d);
 }
+LYTH_D float2 mx_mul2_rz(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rz.f32x2 %0, %1, %2;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
 LYTH_D float2 mx_add2(float2 a, float2 b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;"
@@ -427,6 +434,49 @@ LYTH_D float2 mx_fma2(float2 a, float2 b, float2 c) {
         : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)),
           "l"(*reinterpret_cast<uint64_t *>(&c)));
     return *reinterpret_cast<float2 *>(&d);
+}
+
+// Two products rounded to odd: cut, and the last bit set where the cut lost something (or is NaN). Rounding that
+// to a shorter type is rounding the product itself to it. The products' last bits are f32 numbers here.
+LYTH_D float2 mx_mul2_odd(float2 a, float b) {
+    const float2 v = mx_mul2_rz(a, make_float2(b, b)), lost = mx_fma2(a, make_float2(-b, -b), v);
+    return make_float2(__uint_as_float(__float_as_uint(v.x) | (lost.x != 0.0f)),
+                       __uint_as_float(__float_as_uint(v.y) | (lost.y != 0.0f)));
+}
+// The sixteen values of an NVFP4 block in a 16-bit type, each code * s * g rounded once (code * s is exact, and f32
+// before the type would be a second rounding). A block has eight magnitudes: they are rounded once for all, and
+// the values looked up by byte: 14336 x 4096 to bf16 24.0 us, as with two roundings; each value by itself 29.1.
+template <int TY>
+LYTH_D void mx_nvfp4_back(uint32_t w0, uint32_t w1, float s, float g, uint32_t (&out)[8]) {
+    uint32_t m[4];  // the magnitudes of codes 2 i and 2 i + 1
+    if constexpr (TY == LYTH_NARROW_BF16) {
+        // 2^-110 .. 2^112, normal numbers of bf16: s g and 3 s g rounded, the others steps of the exponent from them
+        const float2 v = mx_mul2_odd(make_float2(s, __fmul_rn(s, 3.0f)), g);
+        const uint32_t p = mx_pack2<TY>(v.x, v.y);
+        const bool number = s != 0.0f && s == s;  // else all are zero, or NaN
+        m[0] = number ? (p << 16) - 0x00800000u : p;
+        m[1] = number ? p - 0x00800000u : p;
+        m[2] = number ? p + 0x00000080u : p;
+        m[3] = number ? p + 0x00800100u : p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            constexpr float kCode[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
+            const float2 v = mx_mul2_odd(mx_mul2(make_float2(kCode[2 * i], kCode[2 * i + 1]), make_float2(s, s)), g);
+            m[i] = mx_pack2<TY>(v.x, v.y);
+        }
+    }
+    const uint32_t lo0 = __byte_perm(m[0], m[1], 0x6420), lo1 = __byte_perm(m[2], m[3], 0x6420);
+    const uint32_t hi0 = __byte_perm(m[0], m[1], 0x7531), hi1 = __byte_perm(m[2], m[3], 0x7531);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {  // four codes each
+        const uint32_t w = (i & 2 ? w1 : w0) >> (16 * (i & 1));
+        const uint32_t sign = __byte_perm(w << 4, w, 0x5140);  // of code j in bit 7 of byte j
+        const uint32_t lo = __byte_perm(lo0, lo1, w & 0x7777u);
+        const uint32_t hi = __byte_perm(hi0, hi1, w & 0x7777u) ^ (sign & 0x80808080u);
+        out[2 * i] = __byte_perm(lo, hi, 0x5140);
+        out[2 * i + 1] = __byte_perm(lo, hi, 0x7362);
+    }
 }
 
 // Quantise the sixteen values of chunk c (columns 16 c ..) of a row, `top` the bits of their largest
