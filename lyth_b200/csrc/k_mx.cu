@@ -299,14 +299,16 @@ static MxFlat mx_flat(int fmt, uint64_t rows, uint32_t cols, uint64_t ld, int u,
     f.cpr = (uint32_t)(mx_padded(fmt, cols) / kMxChunk);
     f.step_rows = kMxThreads / f.cpr;
     f.step_c = kMxThreads % f.cpr;
-    const uint64_t per = (uint64_t)kMxThreads * u, blocks = (rows * f.cpr + per - 1) / per;
+    // 2^38 chunks at most, so that the blocks fit a grid; rows * cpr itself may pass 64 bits
+    const uint64_t per = (uint64_t)kMxThreads * u;
+    const uint64_t blocks = rows > (1ull << 38) / f.cpr ? 0 : (rows * f.cpr + per - 1) / per;
     f.narrow = blocks * per <= 0xFFFFFFFFull;
-    grid = blocks < (1ull << 31) ? (unsigned)blocks : 0u;
+    grid = (unsigned)blocks;
     return f;
 }
 
 // What every entry here asks of its sizes: known format and type, columns that a 32-bit index
-// holds after padding, rows whose chunks a 64-bit count holds.
+// holds after padding, rows that a 64-bit byte offset reaches.
 static int mx_shape(int fmt, int ty, uint64_t rows, uint32_t cols) {
     if (!mx_known(fmt) || !mx_ty_known(ty)) return LYTH_E_UNSUPPORTED;
     if (cols == 0 || cols > (1u << 30) || rows > (1ull << 40)) return LYTH_E_INVALID;

@@ -291,3 +291,12 @@ def test_a_format_past_32_bits_is_unknown(on_device0):
     with pytest.raises(lb.LythError) as e:
         lb.quantize_mx(1 << 32, Fake((0, 64), torch.bfloat16), *held(lb.MX_FP8, 0, 64))
     assert e.value.status == lb.E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("call", [quantize, dequantize])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", [(1 << 40, 1 << 30), ((1 << 38) + 1, 1 << 30), ((1 << 39) + 3, (1 << 30) - 5), (1 << 40, 1 << 20)])
+def test_more_chunks_than_a_launch(call, fmt, rows, cols):
+    # rows x columns of 16 whose count passes 64 bits must not come back as a few
+    ld = {"ldx" if call is quantize else "ldo": cols}
+    assert call(fmt=fmt, rows=rows, cols=cols, **ld) == lb.E_INVALID
