@@ -525,7 +525,7 @@ int lyth_b200_reduce_partials_narrow(int op, int ty, uint64_t n, const uint16_t 
  * are taken; those that start on 32 bytes are quickest. Codes and scales start on 16 bytes, other
  * pointers on an element (else LYTH_E_UNSUPPORTED). Zero rows are fine and do nothing. LYTH_E_INVALID:
  * zero columns or over 2^30 (gemv_mx 2^24), over 2^40 rows (matmul_mx 2^31 - 512 of m or n, gemv_mx 2^31
- * of n), over 2^42 values of k columns (quantize_mx, dequantize_mx), a stride below the width, a tensor
+ * of n), over 2^42 values of k columns (quantize_mx, dequantize_mx, rmsnorm_mx), a stride below the width, a tensor
  * scale outside 2^-100 .. 2^100 (MX formats: other than 1).
  * Outputs overlap no input and no other output, but for residual_out as stated. No call allocates or
  * keeps anything; all can be captured, and run beside one another on several streams. */

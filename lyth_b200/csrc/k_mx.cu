@@ -290,7 +290,7 @@ extern "C" uint64_t lyth_b200_mx_scale_bytes(int fmt, uint64_t rows, uint32_t co
     return mx_known(fmt) ? (rows + 127) / 128 * (mx_padded(fmt, cols) / (4 * mx_block(fmt))) * 512 : 0;
 }
 
-// Chunks to blocks of kMxThreads * u; grid 0 where they do not fit one launch.
+// Chunks to blocks of kMxThreads * u.
 static MxFlat mx_flat(int fmt, uint64_t rows, uint32_t cols, uint64_t ld, int u, unsigned &grid) {
     MxFlat f;
     f.rows = rows;
@@ -299,19 +299,17 @@ static MxFlat mx_flat(int fmt, uint64_t rows, uint32_t cols, uint64_t ld, int u,
     f.cpr = (uint32_t)(mx_padded(fmt, cols) / kMxChunk);
     f.step_rows = kMxThreads / f.cpr;
     f.step_c = kMxThreads % f.cpr;
-    // 2^38 chunks at most, so that the blocks fit a grid; rows * cpr itself may pass 64 bits
-    const uint64_t per = (uint64_t)kMxThreads * u;
-    const uint64_t blocks = rows > (1ull << 38) / f.cpr ? 0 : (rows * f.cpr + per - 1) / per;
+    const uint64_t per = (uint64_t)kMxThreads * u, blocks = (rows * f.cpr + per - 1) / per;  // 2^30 at most
     f.narrow = blocks * per <= 0xFFFFFFFFull;
     grid = (unsigned)blocks;
     return f;
 }
 
 // What every entry here asks of its sizes: known format and type, columns that a 32-bit index
-// holds after padding, rows that a 64-bit byte offset reaches.
+// holds after padding, no more values than a grid and a byte offset hold (rows * k may pass 64 bits).
 static int mx_shape(int fmt, int ty, uint64_t rows, uint32_t cols) {
     if (!mx_known(fmt) || !mx_ty_known(ty)) return LYTH_E_UNSUPPORTED;
-    if (cols == 0 || cols > (1u << 30) || rows > (1ull << 40)) return LYTH_E_INVALID;
+    if (cols == 0 || cols > (1u << 30) || rows > (1ull << 40) || rows > (1ull << 42) / mx_padded(fmt, cols)) return LYTH_E_INVALID;
     return LYTH_OK;
 }
 
@@ -327,7 +325,6 @@ extern "C" int lyth_b200_quantize_mx(int fmt, int ty, uint64_t rows, uint32_t co
     const bool vec = cols % 16 == 0 && aligned32(x) && ldx * mx_ty_bytes(ty) % 32 == 0;
     unsigned grid;
     const MxFlat f = mx_flat(fmt, rows, cols, ldx, vec ? 2 : 1, grid);
-    if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
                      auto k = vec ? mx_quantize_kernel<FMT, TY, true, 2> : mx_quantize_kernel<FMT, TY, false, 1>;
                      return mx_launch(k, grid, kMxThreads, 0, s, 1, static_cast<const MxElem<TY>::type *>(x), f,
@@ -348,7 +345,6 @@ extern "C" int lyth_b200_dequantize_mx(int fmt, int ty, uint64_t rows, uint32_t 
     const bool vec = cols % 16 == 0 && aligned32(out) && ldo * mx_ty_bytes(ty) % 32 == 0;
     unsigned grid;
     const MxFlat f = mx_flat(fmt, rows, cols, ldo, vec ? 2 : 1, grid);
-    if (grid == 0) return LYTH_E_INVALID;
     LYTH_MX_DISPATCH(fmt, ty,
                      auto k = vec ? mx_dequantize_kernel<FMT, TY, true, 2> : mx_dequantize_kernel<FMT, TY, false, 1>;
                      return mx_launch(k, grid, kMxThreads, 0, s, 1, codes, scales, f, tensor_scale,

@@ -300,3 +300,9 @@ def test_more_chunks_than_a_launch(call, fmt, rows, cols):
     # rows x columns of 16 whose count passes 64 bits must not come back as a few
     ld = {"ldx" if call is quantize else "ldo": cols}
     assert call(fmt=fmt, rows=rows, cols=cols, **ld) == lb.E_INVALID
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", [(1 << 40, 1 << 30), ((1 << 38) + 1, 1 << 30), ((1 << 12) + 1, 1 << 30)])
+def test_norm_of_more_values_than_an_offset_reaches(fmt, rows, cols):
+    assert rmsnorm(fmt=fmt, rows=rows, cols=cols, ldx=cols, ldr=cols, ldo=cols) == lb.E_INVALID
