@@ -517,16 +517,18 @@ int lyth_b200_reduce_partials_narrow(int op, int ty, uint64_t n, const uint16_t 
  * the last are neither written nor used. A code stands for code * scale (* tensor scale).
  * Quantisation: the MX scale is the exponent of the block's largest magnitude less that of the
  * largest code (at least 2^-127); the NVFP4 scale is that magnitude / (6 * tensor_scale) rounded to
- * E4M3 (at most 448). Codes are value / scale rounded to nearest even and saturated; a block whose
- * scale rounds to zero gets zero codes, one that holds an infinity or a NaN the NaN scale (0xFF,
- * 0x7F) and zero codes.
+ * E4M3 (at most 448). Codes are value / scale rounded to nearest even and saturated. MX quotients are
+ * exact. NVFP4's are taken in f32 and off by 2^-23 of themselves at most, so one nearer than that to
+ * halfway between two results may become either; for 16-bit values under a tensor scale that is a power of
+ * two both are the exact quotients'. A block whose scale rounds to zero gets zero codes, one that holds an
+ * infinity or a NaN the NaN scale (0xFF, 0x7F) and zero codes.
  * `ty` is the type of the unquantised side: LYTH_MX_F32, LYTH_NARROW_F16 or LYTH_NARROW_BF16. Row
  * strides (ld*) count elements, and what lies between rows is left as it was. Rows of any alignment
  * are taken; those that start on 32 bytes are quickest. Codes and scales start on 16 bytes, other
  * pointers on an element (else LYTH_E_UNSUPPORTED). Zero rows are fine and do nothing. LYTH_E_INVALID:
  * zero columns or over 2^30 (gemv_mx 2^24), over 2^40 rows (matmul_mx 2^31 - 512 of m or n, gemv_mx 2^31
- * of n), over 2^42 values of k columns (quantize_mx, dequantize_mx, rmsnorm_mx), a stride below the width, a tensor
- * scale outside 2^-100 .. 2^100 (MX formats: other than 1).
+ * of n), over 2^42 values of k columns (quantize_mx, dequantize_mx, rmsnorm_mx), a stride below the width,
+ * a tensor scale outside 2^-100 .. 2^100 (MX formats: other than 1).
  * Outputs overlap no input and no other output, but for residual_out as stated. No call allocates or
  * keeps anything; all can be captured, and run beside one another on several streams. */
 #define LYTH_MX_FP8 0
@@ -550,13 +552,13 @@ int lyth_b200_rmsnorm_mx(int fmt, int ty, uint64_t rows, uint32_t cols, const vo
                          const void *residual, uint64_t ldr, void *residual_out, uint64_t ldo, const void *weight,
                          float eps, float tensor_scale, uint8_t *codes, uint8_t *scales, cudaStream_t stream);
 /* c (m x n of `ty`) = alpha * a b^T: a is m x cols, b n x cols, both in `fmt`; f32 accumulation on
- * the block-scaled tensor cores (tcgen05.mma .block_scale), rounded once. alpha carries the tensor
- * scales. Any m, n, cols; m or n zero does nothing. */
+ * the block-scaled tensor cores (tcgen05.mma .block_scale), the sum times alpha in f32, rounded to the type.
+ * alpha carries the tensor scales. Any m, n, cols; m or n zero does nothing. */
 int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint32_t cols, const uint8_t *a,
                         const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, float alpha, void *c,
                         uint64_t ldc, cudaStream_t stream);
 /* y (m x n) = alpha * x w^T for a few rows of unquantised x: x is m x cols of `ty` (f16 or bf16),
- * m <= LYTH_GEMV_MX_MAX_M, w n x cols in `fmt`; f32 accumulation, y rounded once to `ty`. A row of y
+ * m <= LYTH_GEMV_MX_MAX_M, w n x cols in `fmt`; f32 accumulation, the sum times alpha in f32, rounded to `ty`. A row of y
  * does not depend on what the other rows of x hold. bf16 x is brought into f16's range by 128 columns
  * (E4M3 weights: 64) of a row at a time, by a power of two: values below 2^-31 of the largest among
  * them lose bits; all other products are exact before the f32 sums, whatever the block scales. */
