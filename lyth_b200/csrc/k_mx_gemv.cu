@@ -22,6 +22,7 @@
 //                        teams 10.6). The partial sums of a group stay in shared memory, where all meet once
 //                        at the end and add them up in a fixed order. Where x does not fit, k is walked
 //                        in chunks, x staged chunk by chunk.
+// At the 96 registers that 640 threads leave, every bf16 instance spills (16 to 72 bytes of stores), no f16 one.
 // Every mbarrier wait is bounded (mbar.cuh); one that runs out sets the device error flag and the
 // block winds down. Loading and converting in the same warps, with four steps of loads in flight in
 // registers, took 13.2 us for one token through 14336 x 4096 NVFP4 weights: 9.5 us without the loads,

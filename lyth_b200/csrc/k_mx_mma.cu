@@ -880,7 +880,10 @@ extern "C" int lyth_b200_matmul_mx(int fmt, int ty, uint32_t m, uint32_t n, uint
     p.alpha = alpha;
     p.vec = aligned32(c) && ldc * mx_ty_bytes(ty) % 32 == 0;
     p.vec4 = ((uintptr_t)c & (4 * mx_ty_bytes(ty) - 1)) == 0 && ldc % 4 == 0;
-    // one tile per SM at most: single SMs, else pairs
+    // one tile per SM at most: single SMs, else pairs. us on single SMs and on pairs, NVFP4, k 4096: 32 x 18944
+    // (148 tiles) 10.3 and 13.6, 32 x 19072 (149) 15.7 and 15.0; 1024 x 2304 (144) 7.7 and 9.9, 1024 x 2432 (152)
+    // 13.8 and 9.7. (Where few rows fill a second round of single SMs well it is the other way: 32 x 28672 x
+    // 8192, 224 tiles, 28.2 and 30.5.)
     const uint64_t tiles = ((uint64_t)m + XM_BM - 1) / XM_BM * (((uint64_t)n + XM_BN - 1) / XM_BN);
     if (tiles > (uint64_t)device_sms()) {
         // The tiles' width by the rounds that all pairs make over them: of 192, 256 or 384 columns, a column
