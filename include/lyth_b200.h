@@ -518,7 +518,7 @@ int lyth_b200_reduce_partials_narrow(int op, int ty, uint64_t n, const uint16_t 
  * Quantisation: the MX scale is the exponent of the block's largest magnitude less that of the
  * largest code (at least 2^-127); the NVFP4 scale is that magnitude / (6 * tensor_scale) rounded to
  * E4M3 (at most 448). Codes are value / scale rounded to nearest even and saturated. MX quotients are
- * exact. NVFP4's are taken in f32 and off by 2^-23 of themselves at most, so one nearer than that to
+ * exact. NVFP4's are taken in f32 and off by less than 2^-22 of themselves, so one nearer than that to
  * halfway between two results may become either; for 16-bit values under a tensor scale that is a power of
  * two both are the exact quotients'. A block whose scale rounds to zero gets zero codes, one that holds an
  * infinity or a NaN the NaN scale (0xFF, 0x7F) and zero codes.

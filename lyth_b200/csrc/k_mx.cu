@@ -5,7 +5,7 @@
 // scale byte are written. A thread holds sixteen consecutive values: an NVFP4 block, or half an MX
 // block whose other half is the neighbouring lane's (mx_quantize), so no value is read twice and
 // shared memory is used only for the norm's row sum. Measured: 14336 x 4096 bf16 to NVFP4 27.1 us (150
-// MB, 5.6 TB/s), back 24.3 (6.2); f32 24.6 us of 8192 x 4096 (6.2); the norm of 8192 x 4096 bf16 with a
+// MB, 5.6 TB/s), back 24.0 (6.3); f32 24.6 us of 8192 x 4096 (6.2); the norm of 8192 x 4096 bf16 with a
 // residual to MXFP8 38.3 us (236 MB, 6.2 TB/s). Rows that do not start on 32 bytes cost up to twice the
 // norm's time (8192 x 4099: 67 us), in the instructions that shift them.
 #include "mx.cuh"

@@ -500,7 +500,7 @@ LYTH_D void mx_quantize(const float (&v)[16], uint32_t top, bool live, uint32_t 
         // 1 / d in two parts, the first rounded down: v r + (v r_lo) is v / d to 2^-46, rounded once, so
         // values halfway between two codes are halfway here too (v r alone misses some of them when d
         // is 13, 14 or 15 eighths of a power of two). d is rounded itself unless g is a power of two; then
-        // a quotient is off by 2^-23 at most. r_lo >= 0 keeps the sign of a zero.
+        // a quotient is off by less than 2^-22. r_lo >= 0 keeps the sign of a zero.
         const float d = __fmul_rn(mx_scales2<FMT>(byte).x, g), r = byte == 0 ? 0.0f : __frcp_rd(d);
         const float r_lo = __fmul_rn(__fmaf_rn(-d, r, 1.0f), r);
 #pragma unroll
